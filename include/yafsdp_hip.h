@@ -47,7 +47,8 @@ typedef enum yafsdp_status {
   YAFSDP_ERR_OUT_OF_MEMORY = -5,
   YAFSDP_ERR_TOO_LARGE = -6,
   YAFSDP_ERR_BUSY = -7,
-  YAFSDP_ERR_UNSUPPORTED = -8
+  YAFSDP_ERR_UNSUPPORTED = -8,
+  YAFSDP_ERR_OVERLAP = -9
 } yafsdp_status;
 
 /* per-tensor mode of yafsdp_gather_in / yafsdp_scatter_out / fragments */
@@ -388,6 +389,66 @@ enum { YAFSDP_ADAM_DECOUPLED_DECAY = 1, YAFSDP_ADAM_ZERO_GRAD = 2 };
 int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_sq, void* out16, int out16_dtype,
                       int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
                       int64_t step, const float* grad_scale, int flags, void* stream);
+
+/* ---- the same passes over a list of separate tensors ----------------------------
+ * For tensors that are not ranges of one flat buffer: parameters outside any
+ * group, gradients as autograd leaves them, fragments of several groups at once,
+ * in any mixture of the three dtypes.  The reference runs these as torch foreach
+ * ops over the list (torch.nn.utils.clip_grad_norm_, ya_fsdp/_tensor.py:220-262;
+ * _fused_adamw_, :300-312).  The list is a host array; it travels in the kernel
+ * arguments (240 ranges per launch, 80 for AdamW; tensors that follow each other
+ * in memory count as one), so a call keeps no state, needs no staging copy, may
+ * run next to any other on any stream, and can be captured into a HIP graph
+ * (which then holds the addresses).  Entries with numel 0 are skipped whatever
+ * their pointer.  Data is element-aligned; any such address works, 128-byte
+ * aligned starts are fastest. */
+typedef struct yafsdp_list_entry {
+  void* data; /* device pointer; only read by yafsdp_list_norm */
+  int64_t numel;
+  int32_t dtype; /* yafsdp_dtype */
+  int32_t reserved;
+} yafsdp_list_entry;
+
+typedef enum yafsdp_norm { YAFSDP_NORM_1 = 1, YAFSDP_NORM_2 = 2, YAFSDP_NORM_INF = 3 } yafsdp_norm;
+
+/* Bytes of device workspace yafsdp_list_norm and yafsdp_list_clip need (a constant). */
+size_t yafsdp_list_workspace_bytes(void);
+
+/* norm_and_coef[0] = the norm over all elements of all entries (an element in two entries counts twice):
+ *   YAFSDP_NORM_2    sqrt(sum x^2), YAFSDP_NORM_1  sum |x|: in binary64, rounded to binary32 once
+ *   YAFSDP_NORM_INF  max |x|, NaN if any x is NaN
+ * norm_and_coef[1] = min(max_norm / (norm + 1e-6), 1) in binary32 (NaN kept), as yafsdp_clip_coef.  An empty list
+ * has norm 0.  The order of the additions follows from the list's sizes and addresses alone: a call repeated on the
+ * same list gives the same bits.  `workspace` (8-byte aligned) is scratch for the duration of the call on `stream`
+ * and needs no particular contents. */
+int yafsdp_list_norm(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
+                     size_t workspace_bytes, float* norm_and_coef, void* stream);
+
+/* yafsdp_list_norm followed by x = round(float(x) * norm_and_coef[1]) on every element, in place (nothing is
+ * written when the coefficient is exactly 1).  Entries must not share memory (YAFSDP_ERR_OVERLAP, nothing launched). */
+int yafsdp_list_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
+                     size_t workspace_bytes, float* norm_and_coef, void* stream);
+
+/* x = round(float(x) * *coef) on every element, in place, the coefficient read on the device (yafsdp_flat_scale over
+ * a list).  Entries must not share memory (YAFSDP_ERR_OVERLAP, nothing launched). */
+int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* stream);
+
+/* One Adam(W) step on every entry: yafsdp_adamw_step's arithmetic and bits, with gradients in any of the three
+ * dtypes (`grad_dtype`; a 16-bit gradient is used as the binary32 number it stands for) and no alignment rule beyond
+ * the element's.  `out16_dtype` YAFSDP_F32: no 16-bit copy, `out16` ignored.  param, exp_avg and exp_avg_sq are
+ * binary32.  What is written (with YAFSDP_ADAM_ZERO_GRAD that includes the gradients) must not share memory with
+ * anything else of the list (YAFSDP_ERR_OVERLAP, nothing launched). */
+typedef struct yafsdp_adamw_entry {
+  float* param;
+  void* grad;
+  float* exp_avg;
+  float* exp_avg_sq;
+  void* out16;
+  int64_t numel;
+} yafsdp_adamw_entry;
+int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dtype, int out16_dtype, double lr,
+                      double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                      const float* grad_scale, int flags, void* stream);
 
 /* Measurement hook: arms a pair of HIP events (hipEvent_t, created with timing
  * enabled) for the calling thread.  The next kernel this thread launches

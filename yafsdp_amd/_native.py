@@ -74,6 +74,11 @@ EXPORTED_SYMBOLS = (
     "yafsdp_clip_coef",
     "yafsdp_flat_scale",
     "yafsdp_adamw_step",
+    "yafsdp_list_workspace_bytes",
+    "yafsdp_list_norm",
+    "yafsdp_list_clip",
+    "yafsdp_list_scale",
+    "yafsdp_list_adamw",
     "yafsdp_time_next_launch",
     "yafsdp_complete_next_launch",
     "yafsdp_complete_next_launch_pending",
@@ -167,6 +172,16 @@ def _load() -> ctypes.CDLL:
     lib.yafsdp_flat_scale.argtypes = [vp, i32, i64, vp, vp]
     lib.yafsdp_adamw_step.restype = i32
     lib.yafsdp_adamw_step.argtypes = [vp, vp, vp, vp, vp, i32, i64, dbl, dbl, dbl, dbl, dbl, i64, vp, i32, vp]
+    lib.yafsdp_list_workspace_bytes.restype = ctypes.c_size_t
+    lib.yafsdp_list_workspace_bytes.argtypes = []
+    lib.yafsdp_list_norm.restype = i32
+    lib.yafsdp_list_norm.argtypes = [vp, i64, i32, dbl, vp, ctypes.c_size_t, vp, vp]
+    lib.yafsdp_list_clip.restype = i32
+    lib.yafsdp_list_clip.argtypes = [vp, i64, i32, dbl, vp, ctypes.c_size_t, vp, vp]
+    lib.yafsdp_list_scale.restype = i32
+    lib.yafsdp_list_scale.argtypes = [vp, i64, vp, vp]
+    lib.yafsdp_list_adamw.restype = i32
+    lib.yafsdp_list_adamw.argtypes = [vp, i64, i32, i32, dbl, dbl, dbl, dbl, dbl, i64, vp, i32, vp]
     lib.yafsdp_time_next_launch.restype = i32
     lib.yafsdp_time_next_launch.argtypes = [vp, vp]
     lib.yafsdp_complete_next_launch.restype = i32
@@ -195,6 +210,7 @@ def error_string(code: int) -> str:
 
 ERR_BUSY = -7  # YAFSDP_ERR_BUSY: every staging slot of a table is held by a queued call
 ERR_UNSUPPORTED = -8  # YAFSDP_ERR_UNSUPPORTED: a fused entry point does not serve this table / dtype combination
+ERR_OVERLAP = -9  # YAFSDP_ERR_OVERLAP: tensors of a list that the call writes share memory
 
 
 def _check(code: int, what: str) -> None:
@@ -899,6 +915,231 @@ def adamw_step(
             ),
             "yafsdp_adamw_step",
         )
+
+
+# ---- the same passes over a list of separate tensors ---------------------------
+NORM_CODE = {1.0: 1, 2.0: 2, float("inf"): 3}
+LIST_WORKSPACE_BYTES = int(lib.yafsdp_list_workspace_bytes())
+_LIST_ENTRY = np.dtype([("data", np.uint64), ("numel", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
+_ADAMW_ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("exp_avg", np.uint64), ("exp_avg_sq", np.uint64),
+                         ("out16", np.uint64), ("numel", np.int64)])
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one range of memory, each once, in whatever order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size == 1:
+            continue
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _list_device(t: torch.Tensor, what: str, device: torch.device | None) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} must live on the GPU, got {t.device}: this path has no CPU implementation")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{what} on {t.device}, the tensors before it on {device}: one call serves one GPU")
+    return t.device
+
+
+def _as_list(tensors, what: str) -> list:
+    if isinstance(tensors, torch.Tensor):
+        raise TypeError(f"{what}: expected a list of tensors, got a tensor")
+    return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
+
+
+class TensorList:
+    """A list of tensors as the ``yafsdp_list_*`` entry points take it: one entry per tensor, ``None`` left out.  Any
+    mixture of the path's dtypes, any sizes (0 included), on one GPU; each tensor dense (contiguous in some order of
+    its dimensions).  ``resolve`` maps a wrapper subclass to the plain tensor it holds.  Made for one call: it holds
+    addresses."""
+
+    __slots__ = ("tensors", "entries", "count", "device")
+
+    def __init__(self, tensors, what: str = "tensors", resolve=None):
+        tensors = _as_list(tensors, what)
+        got = _tensorlist.list_entries(tensors, True) if _tensorlist is not None else None
+        if got is not None:
+            self.tensors = tensors
+            self.entries, self.count, index = got
+            self.device = torch.device("cuda", index)
+            return
+        # not accepted as it stands: resolve wrappers, find out what is wrong and raise
+        if resolve is not None:
+            tensors = [None if t is None else resolve(t) for t in tensors]
+        rows, device = [], None
+        for i, t in enumerate(tensors):
+            if t is None:
+                continue
+            device = _list_device(t, f"{what}[{i}]", device)
+            if not _is_dense(t) or t.is_neg():
+                raise NotImplementedError(
+                    f"{what}[{i}] must be dense: shape={tuple(t.shape)} stride={t.stride()}")
+            rows.append((t.data_ptr(), t.numel(), _dt(t), 0))
+        if device is None:
+            raise ValueError(f"{what}: no tensors")
+        self.tensors = tensors
+        self.entries, self.count, self.device = np.array(rows, dtype=_LIST_ENTRY).tobytes(), len(rows), device
+
+    def bump_versions(self) -> None:
+        """What an in-place torch op does to its tensors' version counters."""
+        _bump_versions(self.tensors)
+
+
+def _bump_versions(tensors) -> None:
+    if _tensorlist is not None:
+        _tensorlist.bump_versions(tensors)
+    else:
+        torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
+
+
+def norm_code(norm_type) -> int:
+    try:
+        return NORM_CODE[float(norm_type)]
+    except KeyError:
+        raise NotImplementedError(f"only the 1-, 2- and infinity-norm are implemented, got {norm_type}") from None
+
+
+def _check_norm_out(lst: TensorList, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
+    _flat_arg(norm_and_coef, "norm_and_coef"), _flat_arg(workspace, "workspace")
+    if norm_and_coef.dtype != torch.float32 or norm_and_coef.numel() < 2:
+        raise TypeError("norm_and_coef must be float32 with two elements")
+    if norm_and_coef.device != lst.device or workspace.device != lst.device:
+        raise RuntimeError("the tensors, norm_and_coef and workspace must live on one device")
+
+
+def list_workspace(device: torch.device) -> torch.Tensor:
+    """Scratch of ``list_norm`` / ``list_clip``; reusable across calls that do not overlap."""
+    return torch.empty(LIST_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
+
+
+def _list_norm(fn, name, lst, norm_type, max_norm, norm_and_coef, workspace) -> None:
+    code = norm_code(norm_type)
+    _check_norm_out(lst, norm_and_coef, workspace)
+    with _on(lst.device):
+        _check(
+            fn(lst.entries, lst.count, code, float(max_norm), workspace.data_ptr(),
+               workspace.numel() * workspace.element_size(), norm_and_coef.data_ptr(), _stream(norm_and_coef)),
+            name,
+        )
+
+
+def list_norm(lst: TensorList, norm_type, max_norm: float, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
+    """``{norm, clip coefficient}`` (float32) over every element of the list; ``norm_type`` 1, 2 or infinity."""
+    _list_norm(lib.yafsdp_list_norm, "yafsdp_list_norm", lst, norm_type, max_norm, norm_and_coef, workspace)
+
+
+def list_clip(lst: TensorList, norm_type, max_norm: float, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
+    """``list_norm``, then every element times the coefficient, in place."""
+    _list_norm(lib.yafsdp_list_clip, "yafsdp_list_clip", lst, norm_type, max_norm, norm_and_coef, workspace)
+
+
+def list_scale(lst: TensorList, coef: torch.Tensor) -> None:
+    """``t.mul_(coef)`` for every tensor of the list, ``coef`` a one-element float32 device tensor."""
+    _flat_arg(coef, "coef")
+    if coef.dtype != torch.float32 or coef.numel() != 1 or coef.device != lst.device:
+        raise TypeError("coef must be a one-element float32 tensor on the list's device")
+    with _on(lst.device):
+        _check(lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), _stream(coef)), "yafsdp_list_scale")
+
+
+class AdamwList:
+    """Parallel lists of an AdamW step as ``yafsdp_list_adamw`` takes them: float32 ``params``, ``exp_avgs``,
+    ``exp_avg_sqs``; ``grads`` of one dtype (``None``: that position is left out); ``outs16`` (optional) of one 16-bit
+    dtype.  All contiguous, on one GPU.  Made for one call: it holds addresses."""
+
+    __slots__ = ("lists", "entries", "count", "device", "grad_code", "out_code")
+    _NAMES = ("params", "grads", "exp_avgs", "exp_avg_sqs", "outs16")
+
+    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, outs16=None, resolve=None):
+        lists = [_as_list(ts, name) for ts, name in zip((params, grads, exp_avgs, exp_avg_sqs), self._NAMES)]
+        lists.append(None if outs16 is None else _as_list(outs16, "outs16"))
+        got = _tensorlist.adamw_entries(*lists, True) if _tensorlist is not None else None
+        if got is not None:
+            self.lists = lists
+            self.entries, self.count, index, self.grad_code, self.out_code = got
+            self.device = torch.device("cuda", index)
+            return
+        if resolve is not None:
+            lists = [None if ts is None else [None if t is None else resolve(t) for t in ts] for ts in lists]
+        n = len(lists[0])
+        for ts, name in zip(lists, self._NAMES):
+            if ts is not None and len(ts) != n:
+                raise ValueError(f"{name}: expected {n} tensors, got {len(ts)}")
+        rows, device, grad_dtype, out_dtype = [], None, None, None
+        for i in range(n):
+            if lists[1][i] is None:
+                continue
+            row = []
+            for ts, name in zip(lists, self._NAMES):
+                if ts is None:
+                    row.append(0)
+                    continue
+                t, what = ts[i], f"{name}[{i}]"
+                device = _list_device(t, what, device)
+                if not t.is_contiguous() or t.is_neg():
+                    raise NotImplementedError(f"{what} must be contiguous: shape={tuple(t.shape)} stride={t.stride()}")
+                if t.numel() != lists[0][i].numel():
+                    raise ValueError(f"{what}: numel {t.numel()} != {lists[0][i].numel()}")
+                if name == "grads":
+                    _dt(t)
+                    if grad_dtype not in (None, t.dtype):
+                        raise TypeError(f"grads of one call share a dtype, got {grad_dtype} and {t.dtype}")
+                    grad_dtype = t.dtype
+                elif name == "outs16":
+                    if t.dtype not in (torch.bfloat16, torch.float16) or out_dtype not in (None, t.dtype):
+                        raise TypeError(f"{what}: bfloat16 or float16, one dtype for all, got {t.dtype}")
+                    out_dtype = t.dtype
+                elif t.dtype != torch.float32:
+                    raise TypeError(f"{what} must be float32, got {t.dtype}")
+                row.append(t.data_ptr())
+            rows.append((*row, lists[0][i].numel()))
+        if device is None:
+            raise ValueError("no parameter with a gradient")
+        self.lists = lists
+        self.entries, self.count, self.device = np.array(rows, dtype=_ADAMW_ENTRY).tobytes(), len(rows), device
+        self.grad_code, self.out_code = DTYPE_CODE[grad_dtype], 0 if out_dtype is None else DTYPE_CODE[out_dtype]
+
+    def bump_versions(self, zero_grad: bool) -> None:
+        """Of everything the step writes: the positions with a gradient of every list but the gradients (of those too
+        where the step zero-fills them)."""
+        live = [g is not None for g in self.lists[1]]
+        for k, ts in enumerate(self.lists):
+            if ts is not None and (k != 1 or zero_grad):
+                _bump_versions(ts if all(live) else [t for t, on in zip(ts, live) if on])
+
+
+def list_adamw(
+    lst: AdamwList, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: int,
+    decoupled: bool = True, grad_scale: torch.Tensor | None = None, zero_grad: bool = False, allow_overlap: bool = False,
+) -> bool:
+    """One Adam(W) step on every position of the lists, with the bits of ``adamw_step``.  Tensors that the step writes
+    must not share memory: refused, or with ``allow_overlap`` reported by returning False with nothing launched."""
+    gs_ptr = None
+    if grad_scale is not None:
+        _flat_arg(grad_scale, "grad_scale")
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != lst.device:
+            raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
+        gs_ptr = grad_scale.data_ptr()
+    flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
+    with _on(lst.device):
+        stream = _raw_current_stream(lst.device.index) if _raw_current_stream is not None else (
+            torch.cuda.current_stream(lst.device).cuda_stream)
+        code = lib.yafsdp_list_adamw(
+            lst.entries, lst.count, lst.grad_code, lst.out_code, float(lr), float(beta1), float(beta2), float(eps),
+            float(weight_decay), int(step), gs_ptr, flags, stream,
+        )
+    if code == ERR_OVERLAP and allow_overlap:
+        return False
+    _check(code, "yafsdp_list_adamw")
+    return True
 
 
 def time_next_launch(start: torch.cuda.Event | None, stop: torch.cuda.Event | None) -> None:

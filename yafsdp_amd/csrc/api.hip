@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../include/yafsdp_hip.h"
+#include "adam_scalars.h"
 #include "launch.h"
 #include "stage_ring.h"
 #include "tuning.h"
@@ -352,11 +353,13 @@ const char* yafsdp_error_string(int code) {
     case YAFSDP_ERR_UNSUPPORTED:
       return "yafsdp: this fused entry point does not serve the dtype combination (a reduce buffer that has neither "
              "the gradients' dtype nor binary32): use the two separate entry points";
+    case YAFSDP_ERR_OVERLAP: return "yafsdp: tensors of the list that the call writes share memory";
     case YAFSDP_ERR_BUSY:
       return "yafsdp: every staging slot of this table is still in use by a queued call (more than 8 different "
              "tensor sets in flight): synchronise the stream, or bind tensor sets that persist";
     case YAFSDP_ERR_TOO_LARGE:
-      return "yafsdp: more elements than the entry point's fixed scratch is specified for (yafsdp_flat_sumsq_static: 2^31)";
+      return "yafsdp: more elements than the entry point's fixed scratch is specified for (yafsdp_flat_sumsq_static: "
+             "2^31), or than a list entry point takes";
     default: break;
   }
   if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));
@@ -770,31 +773,7 @@ int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_
       (grad_scale != nullptr && !aligned_to(grad_scale, 4)))
     return YAFSDP_ERR_MISALIGNED;
   const int head = head_elems(param, 4, n);
-  // scalars exactly as torch.optim computes them: Python floats (binary64),
-  // rounded to binary32 where they enter a tensor op
-  AdamScalars s;
-  std::memset(&s, 0, sizeof(s));
-  s.flags = 0;
-  if (weight_decay != 0.0) {
-    if (flags & YAFSDP_ADAM_DECOUPLED_DECAY) {
-      s.flags |= ADAM_DECOUPLED;
-      s.decay = static_cast<float>(1.0 - lr * weight_decay);
-    } else {
-      s.flags |= ADAM_L2;
-      s.l2 = static_cast<float>(weight_decay);
-    }
-  }
-  s.w = static_cast<float>(1.0 - beta1);
-  s.w_m1 = s.w - 1.0f;
-  if (std::fabs(s.w) < 0.5f) s.flags |= ADAM_W_SMALL;
-  s.beta2 = static_cast<float>(beta2);
-  s.one_m_beta2 = static_cast<float>(1.0 - beta2);
-  const double bc1 = 1.0 - std::pow(beta1, double(step));
-  const double bc2 = 1.0 - std::pow(beta2, double(step));
-  s.bc2_sqrt = static_cast<float>(std::pow(bc2, 0.5));
-  s.eps = static_cast<float>(eps);
-  s.neg_step = static_cast<float>(-(lr / bc1));
-  if (flags & YAFSDP_ADAM_ZERO_GRAD) s.flags |= ADAM_ZERO_GRAD;
+  const AdamScalars s = adam_scalars(lr, beta1, beta2, eps, weight_decay, step, flags);
   const int grid = opt_grid((n - head) >> 2, kAdamBlock, kAdamUnroll, nullptr);
   return int(launch_adamw(out16_dtype, param, grad, exp_avg, exp_avg_sq, out16, n, head, s, grad_scale, grid,
                           static_cast<hipStream_t>(stream)));

@@ -5,6 +5,7 @@
 #include <hip/hip_ext.h>
 #include <stdint.h>
 
+#include "list_args.h"
 #include "table_kernels.hip.h"
 
 namespace yafsdp {
@@ -123,5 +124,15 @@ hipError_t launch_sumsq_reduce(const double* in, int64_t count, double* out, int
 hipError_t launch_clip_coef(const double* sumsq, float max_norm, float* norm_and_coef, hipStream_t stream);
 hipError_t launch_adamw(int out_dt, float* p, float* g, float* m, float* v, void* out16, int64_t n, int head,
                         const AdamScalars& s, const float* grad_scale, int grid, hipStream_t stream);
+
+// passes over a list of tensors (list.hip)
+// partials[0:grid] = per-workgroup shares of the norm (LIST_NORM_*)
+hipError_t launch_list_norm(int norm, const ListArgs& a, double* partials, int grid, hipStream_t stream);
+hipError_t launch_list_finish(int norm, const double* partials, int count, float max_norm, float* norm_and_coef,
+                              hipStream_t stream);
+hipError_t launch_list_scale(const ListArgs& a, const float* coef, int grid, hipStream_t stream);
+// out_dt F32: no 16-bit copy of the parameters
+hipError_t launch_list_adamw(int grad_dt, int out_dt, const ListAdamArgs& a, const AdamScalars& s,
+                             const float* grad_scale, int grid, hipStream_t stream);
 
 }  // namespace yafsdp

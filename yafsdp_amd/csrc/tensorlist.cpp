@@ -13,6 +13,9 @@
 #include <torch/extension.h>
 
 #include <cstdint>
+#include <string>
+
+#include "../../include/yafsdp_hip.h"
 
 namespace {
 
@@ -93,10 +96,109 @@ bool all_contiguous(py::handle tensors) {
   return true;
 }
 
+// ---- lists of tensors (yafsdp_list_norm / _clip / _scale / _adamw) ---------------------------------------------
+// A plain torch.Tensor or Parameter in one of the path's dtypes on the wanted kind of device; anything else (wrapper
+// subclasses among them) is left to the Python side.
+inline const at::Tensor* plain_tensor(PyObject* o, bool want_cuda, int64_t& device_index) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.layout() != at::kStrided || t.is_neg()) return nullptr;
+  const auto dev = t.device();
+  if (want_cuda ? !dev.is_cuda() : !dev.is_cpu()) return nullptr;
+  if (device_index == -2) device_index = dev.index();
+  return dev.index() == device_index ? &t : nullptr;
+}
+
+// (entries, count, device index) of a list of tensors, None entries left out; None if the list is not accepted as it
+// stands.  Elementwise and order-free passes: any dense layout will do, whatever its dimension order.
+py::object list_entries(py::handle tensors, bool want_cuda) {
+  PyObject* seq = tensors.ptr();
+  if (!PyList_Check(seq) && !PyTuple_Check(seq)) return py::none();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  PyObject** items = PySequence_Fast_ITEMS(seq);
+  std::string buf(size_t(n) * sizeof(yafsdp_list_entry), '\0');
+  auto* out = reinterpret_cast<yafsdp_list_entry*>(&buf[0]);
+  int64_t device_index = -2, count = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (items[i] == Py_None) continue;
+    const at::Tensor* t = plain_tensor(items[i], want_cuda, device_index);
+    if (t == nullptr) return py::none();
+    const int code = dtype_code(t->scalar_type());
+    if (code < 0 || !t->is_non_overlapping_and_dense()) return py::none();
+    out[count++] = yafsdp_list_entry{t->numel() ? t->data_ptr() : nullptr, t->numel(), code, 0};
+  }
+  if (count == 0) return py::none();
+  return py::make_tuple(py::bytes(buf.data(), size_t(count) * sizeof(yafsdp_list_entry)), count, device_index);
+}
+
+// (entries, count, device index, gradient dtype code, 16-bit copy's dtype code or 0) of five parallel lists; positions
+// without a gradient are left out.  `outs`: None for "no 16-bit copies".  None if not accepted as they stand.
+py::object adamw_entries(py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs,
+                         py::handle outs, bool want_cuda) {
+  const bool has_out = !outs.is_none();
+  PyObject* seqs[5] = {params.ptr(), grads.ptr(), exp_avgs.ptr(), exp_avg_sqs.ptr(), outs.ptr()};
+  const int lists = has_out ? 5 : 4;
+  PyObject** items[5] = {};
+  Py_ssize_t n = -1;
+  for (int k = 0; k < lists; ++k) {
+    if (!PyList_Check(seqs[k]) && !PyTuple_Check(seqs[k])) return py::none();
+    if (n >= 0 && PySequence_Fast_GET_SIZE(seqs[k]) != n) return py::none();
+    n = PySequence_Fast_GET_SIZE(seqs[k]);
+    items[k] = PySequence_Fast_ITEMS(seqs[k]);
+  }
+  std::string buf(size_t(n) * sizeof(yafsdp_adamw_entry), '\0');
+  auto* out = reinterpret_cast<yafsdp_adamw_entry*>(&buf[0]);
+  int64_t device_index = -2, count = 0;
+  int grad_code = -1, out_code = 0;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (items[1][i] == Py_None) continue;
+    const at::Tensor* t[5] = {};
+    for (int k = 0; k < lists; ++k) {
+      t[k] = plain_tensor(items[k][i], want_cuda, device_index);
+      if (t[k] == nullptr || t[k]->numel() != t[0]->numel() || !t[k]->is_contiguous()) return py::none();
+    }
+    for (int k : {0, 2, 3})
+      if (t[k]->scalar_type() != at::kFloat) return py::none();
+    const int g = dtype_code(t[1]->scalar_type());
+    if (g < 0 || (grad_code >= 0 && g != grad_code)) return py::none();
+    grad_code = g;
+    if (has_out) {
+      const int o = dtype_code(t[4]->scalar_type());
+      if (o <= 0 || (out_code > 0 && o != out_code)) return py::none();
+      out_code = o;
+    }
+    const int64_t numel = t[0]->numel();
+    if (numel == 0) continue;
+    out[count++] = yafsdp_adamw_entry{static_cast<float*>(t[0]->data_ptr()), t[1]->data_ptr(),
+                                      static_cast<float*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
+                                      has_out ? t[4]->data_ptr() : nullptr, numel};
+  }
+  if (grad_code < 0) return py::none();
+  return py::make_tuple(py::bytes(buf.data(), size_t(count) * sizeof(yafsdp_adamw_entry)), count, device_index,
+                        grad_code, out_code);
+}
+
+// What an in-place torch op does to its tensors' version counters (the kernels write behind autograd's back).
+void bump_versions(py::handle tensors) {
+  PyObject* seq = tensors.ptr();
+  if (!PyList_Check(seq) && !PyTuple_Check(seq)) throw py::type_error("expected a list or tuple of tensors");
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  PyObject** items = PySequence_Fast_ITEMS(seq);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (items[i] == Py_None) continue;
+    if (!THPVariable_Check(items[i])) throw py::type_error("expected a list or tuple of tensors");
+    const at::Tensor& t = THPVariable_Unpack(items[i]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tensorlist, m) {
   m.attr("REJECTED") = kRejected;
   m.def("fill", &fill, "validate a tensor list against a table and write its pointer / mode arrays");
   m.def("all_contiguous", &all_contiguous);
+  m.def("list_entries", &list_entries, "yafsdp_list_entry array of a list of tensors");
+  m.def("adamw_entries", &adamw_entries, "yafsdp_adamw_entry array of parallel lists of tensors");
+  m.def("bump_versions", &bump_versions);
 }

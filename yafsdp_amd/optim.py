@@ -18,6 +18,22 @@ reference                                      here
 copy-in cast (ya_fsdp/_collectives.py:53-54)    ``adamw_step``
 =============================================  ==============================
 
+Tensors that are not ranges of a group's flat shard (parameters outside any
+group, gradients as autograd leaves them) take the ``list_*`` functions: the same
+passes over a list of separate tensors, in any mixture of float32, bfloat16 and
+float16, a few launches per call:
+
+=============================================  ==============================
+torch                                          here
+=============================================  ==============================
+``torch.nn.utils.get_total_norm``              ``list_grad_norm``
+norm + clip coefficient, gradients untouched   ``list_clip_coef``
+``torch.nn.utils.clip_grad_norm_``             ``list_clip_grad_norm_``
+functional ``adamw`` over parallel lists       ``list_adamw_step``
+=============================================  ==============================
+
+``FlatAdamW`` steps its parameters outside any group through the same list pass.
+
 There is no torch fallback: parameters must be float32 CUDA tensors.
 """
 
@@ -31,11 +47,12 @@ import torch.nn as nn
 from . import _native
 from ._param import YaFSDPParam
 from ._param_group import YaFSDPParamGroup
-from ._tensor import local_tensor
+from ._tensor import local_tensor, plain_tensor
 from ._state import _get_module_fsdp_state
 
 __all__ = ["FlatAdamW", "clip_grad_norm_", "grad_clip_coef", "zero_grad", "fsdp_param_groups",
-           "enable_fused_grad_norm", "disable_fused_grad_norm"]
+           "enable_fused_grad_norm", "disable_fused_grad_norm", "list_grad_norm", "list_clip_coef",
+           "list_clip_grad_norm_", "list_adamw_step"]
 
 
 def fsdp_param_groups(modules: nn.Module | Iterable[nn.Module]) -> list[YaFSDPParamGroup]:
@@ -263,6 +280,84 @@ def zero_grad(modules: nn.Module | Iterable[nn.Module]) -> None:
         _native.flat_fill(group._padded_sharded_param_grad[key], 0.0)
 
 
+def _resolve(t: torch.Tensor) -> torch.Tensor:
+    """The plain tensor behind a sharded parameter or gradient: this rank's fragment."""
+    return plain_tensor(local_tensor(t)) if isinstance(t, torch.Tensor) else t
+
+
+def list_clip_coef(
+    grads: Iterable[torch.Tensor | None], max_norm: float, norm_type: float = 2.0
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(total_norm, clip_coef)`` of a list of gradients as float32 device scalars, without touching them:
+    ``clip_coef = min(max_norm / (total_norm + 1e-6), 1)``.  Pass ``clip_coef`` to ``list_adamw_step`` or
+    ``FlatAdamW.step`` to fuse the scaling into the optimizer pass.
+
+    ``grads`` may mix float32, bfloat16 and float16; ``None`` entries (parameters without a gradient) are left out, and
+    a sharded gradient counts with this rank's fragment.  Each is dense in memory, all live on one GPU.  ``norm_type``
+    is 1, 2 or infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64
+    and are reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls;
+    the call can be captured into a HIP graph, which then reads the same addresses at every replay."""
+    lst = _native.TensorList(grads, "grads", _resolve)
+    norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
+    _native.list_norm(lst, norm_type, max_norm, norm_and_coef, _native.list_workspace(lst.device))
+    return norm_and_coef[0], norm_and_coef[1]
+
+
+def list_grad_norm(grads: Iterable[torch.Tensor | None], norm_type: float = 2.0) -> torch.Tensor:
+    """The total norm of ``list_clip_coef`` (``torch.nn.utils.get_total_norm``)."""
+    return list_clip_coef(grads, 1.0, norm_type)[0]
+
+
+def list_clip_grad_norm_(
+    grads: Iterable[torch.Tensor | None], max_norm: float, norm_type: float = 2.0
+) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` over a list of gradients (see ``list_clip_coef``): every element is multiplied
+    by the clip coefficient in binary32 and rounded to its tensor's dtype, in place; returns the total norm.  Nothing is
+    written when nothing is clipped.  The tensors must not share memory."""
+    lst = _native.TensorList(grads, "grads", _resolve)
+    norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
+    _native.list_clip(lst, norm_type, max_norm, norm_and_coef, _native.list_workspace(lst.device))
+    lst.bump_versions()
+    return norm_and_coef[0]
+
+
+@torch.no_grad()
+def list_adamw_step(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor | None],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    outs16: Sequence[torch.Tensor] | None = None,
+    *,
+    step: int,
+    lr: float = 1e-3,
+    betas: tuple[float, float] = (0.9, 0.999),
+    eps: float = 1e-8,
+    weight_decay: float = 1e-2,
+    decoupled_weight_decay: bool = True,
+    grad_scale: torch.Tensor | None = None,
+    zero_grad: bool = False,
+) -> None:
+    """One AdamW (or, with ``decoupled_weight_decay=False``, Adam) step over parallel lists of tensors, in place.
+
+    ``params`` and both moments are float32; the gradients share one of float32, bfloat16 and float16, and a position
+    without one (``None``) is left as it is.  ``outs16`` (bfloat16 or float16) receives the updated parameters rounded
+    once: masters and moments in float32 next to a 16-bit model.  ``step`` is the 1-based count of the step about to be
+    made.  ``grad_scale`` (one-element float32 device tensor, e.g. from ``list_clip_coef``) multiplies every gradient
+    first, in binary32, without writing it back; ``zero_grad=True`` zero-fills the gradients in the same pass.  Per
+    element the arithmetic is that of ``FlatAdamW``, bit for bit.  All tensors are contiguous, live on one GPU, and what
+    is written shares no memory with anything else in the lists."""
+    if step < 1:
+        raise ValueError(f"Invalid step: {step}")
+    lst = _native.AdamwList(params, grads, exp_avgs, exp_avg_sqs, outs16, _resolve)
+    _native.list_adamw(
+        lst, lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, step=step,
+        decoupled=decoupled_weight_decay, grad_scale=None if grad_scale is None else grad_scale.view(1),
+        zero_grad=zero_grad,
+    )
+    lst.bump_versions(zero_grad)
+
+
 class _Unit:
     """The parameters of one optimizer param group that live in one flat shard
     (an fsdp parameter group), or one plain tensor outside any group."""
@@ -391,23 +486,38 @@ class FlatAdamW(torch.optim.Optimizer):
             beta1, beta2 = pg["betas"]
             hyper = dict(lr=float(pg["lr"]), beta1=beta1, beta2=beta2, eps=pg["eps"],
                          weight_decay=pg["weight_decay"], decoupled=pg["decoupled_weight_decay"])
+            plain: list[_Unit] = []
             for unit in self._units_of(pg_index, pg):
-                self._step_unit(unit, hyper, grad_scale, zero_grad)
+                if unit.group is None:
+                    plain.append(unit)
+                else:
+                    self._step_unit(unit, hyper, grad_scale, zero_grad)
+            if plain:
+                self._step_plain(plain, hyper, grad_scale, zero_grad)
         return loss
+
+    def _step_plain(self, units: list[_Unit], hyper: dict[str, Any], grad_scale, zero_grad: bool) -> None:
+        """Parameters outside any group: one list pass per GPU and step count."""
+        live = [(unit, unit.params[0], unit.params[0].grad) for unit in units if unit.params[0].grad is not None]
+        for _, _, grad in live:
+            if grad.dtype != torch.float32 or not grad.is_contiguous():
+                raise TypeError("FlatAdamW needs contiguous float32 gradients")
+        runs: dict[tuple[torch.device, int], list[tuple[_Unit, torch.Tensor, torch.Tensor]]] = {}
+        for unit, p, grad in live:
+            unit.steps[0] += 1
+            runs.setdefault((unit.device, unit.steps[0]), []).append((unit, p, grad))
+        for (_, step), run in runs.items():
+            lst = _native.AdamwList([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
+                                    [u.exp_avg_sq for u, _, _ in run], None, _resolve)
+            if _native.list_adamw(lst, step=step, grad_scale=grad_scale, zero_grad=zero_grad, allow_overlap=True, **hyper):
+                continue
+            # parameters (or zero-filled gradients) that share memory: one after the other, in the list's order
+            for unit, p, grad in run:
+                _native.adamw_step(p.view(-1), grad.view(-1), unit.exp_avg, unit.exp_avg_sq, None, step=step,
+                                   grad_scale=grad_scale, zero_grad=zero_grad, **hyper)
 
     def _step_unit(self, unit: _Unit, hyper: dict[str, Any], grad_scale, zero_grad: bool) -> None:
         group = unit.group
-        if group is None:
-            (p,) = unit.params
-            if p.grad is None:
-                return
-            unit.steps[0] += 1
-            grad = p.grad
-            if grad.dtype != torch.float32 or not grad.is_contiguous():
-                raise TypeError("FlatAdamW needs contiguous float32 gradients")
-            _native.adamw_step(p.view(-1), grad.view(-1), unit.exp_avg, unit.exp_avg_sq, None,
-                               step=unit.steps[0], grad_scale=grad_scale, zero_grad=zero_grad, **hyper)
-            return
         key = unit.key
         shard = group._padded_sharded_param_data[key]
         grad_shard = group._padded_sharded_param_grad[key]
