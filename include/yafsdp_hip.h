@@ -395,13 +395,18 @@ int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_
  * group, gradients as autograd leaves them, fragments of several groups at once,
  * in any mixture of the three dtypes.  The reference runs these as torch foreach
  * ops over the list (torch.nn.utils.clip_grad_norm_, ya_fsdp/_tensor.py:220-262;
- * _fused_adamw_, :300-312).  The list is a host array; it travels in the kernel
- * arguments (240 ranges per launch, 80 for AdamW; tensors that follow each other
- * in memory count as one), so a call keeps no state, needs no staging copy, may
- * run next to any other on any stream, and can be captured into a HIP graph
- * (which then holds the addresses).  Entries with numel 0 are skipped whatever
- * their pointer.  Data is element-aligned; any such address works, 128-byte
- * aligned starts are fastest. */
+ * _fused_adamw_, :300-312).  The list is a host array that the call is done with
+ * when it returns.  It reaches the GPU in kernel arguments (240 ranges fit in
+ * one launch, 80 of AdamW; longer lists are written to the workspace by small
+ * launches first; tensors that follow each other in memory count as one range),
+ * so a call keeps no state, copies nothing from host memory, may run next to any
+ * other on any stream, and can be captured into a HIP graph (which then holds
+ * the addresses).  `workspace` (16-byte aligned device memory) is scratch for the
+ * duration of the call on `stream` and needs no particular contents; its size is
+ * a function of the number of entries.  Entries with numel 0 are skipped
+ * whatever their pointer.  Data is element-aligned; any such address works,
+ * 128-byte aligned starts are fastest.  Lists of 2^31 tiles (8 TB; 2^39
+ * elements for AdamW) or more are refused (YAFSDP_ERR_TOO_LARGE). */
 typedef struct yafsdp_list_entry {
   void* data; /* device pointer; only read by yafsdp_list_norm */
   int64_t numel;
@@ -411,16 +416,17 @@ typedef struct yafsdp_list_entry {
 
 typedef enum yafsdp_norm { YAFSDP_NORM_1 = 1, YAFSDP_NORM_2 = 2, YAFSDP_NORM_INF = 3 } yafsdp_norm;
 
-/* Bytes of device workspace yafsdp_list_norm and yafsdp_list_clip need (a constant). */
-size_t yafsdp_list_workspace_bytes(void);
+/* Bytes of workspace for n entries: of yafsdp_list_norm, yafsdp_list_clip and yafsdp_list_scale (never 0), and of
+ * yafsdp_list_adamw (0 up to 80 entries: `workspace` may then be NULL). */
+size_t yafsdp_list_workspace_bytes(int64_t n);
+size_t yafsdp_list_adamw_workspace_bytes(int64_t n);
 
 /* norm_and_coef[0] = the norm over all elements of all entries (an element in two entries counts twice):
  *   YAFSDP_NORM_2    sqrt(sum x^2), YAFSDP_NORM_1  sum |x|: in binary64, rounded to binary32 once
  *   YAFSDP_NORM_INF  max |x|, NaN if any x is NaN
  * norm_and_coef[1] = min(max_norm / (norm + 1e-6), 1) in binary32 (NaN kept), as yafsdp_clip_coef.  An empty list
  * has norm 0.  The order of the additions follows from the list's sizes and addresses alone: a call repeated on the
- * same list gives the same bits.  `workspace` (8-byte aligned) is scratch for the duration of the call on `stream`
- * and needs no particular contents. */
+ * same list gives the same bits. */
 int yafsdp_list_norm(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
                      size_t workspace_bytes, float* norm_and_coef, void* stream);
 
@@ -431,7 +437,8 @@ int yafsdp_list_clip(const yafsdp_list_entry* entries, int64_t n, int norm, doub
 
 /* x = round(float(x) * *coef) on every element, in place, the coefficient read on the device (yafsdp_flat_scale over
  * a list).  Entries must not share memory (YAFSDP_ERR_OVERLAP, nothing launched). */
-int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* stream);
+int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* One Adam(W) step on every entry: yafsdp_adamw_step's arithmetic and bits, with gradients in any of the three
  * dtypes (`grad_dtype`; a 16-bit gradient is used as the binary32 number it stands for) and no alignment rule beyond
@@ -448,7 +455,7 @@ typedef struct yafsdp_adamw_entry {
 } yafsdp_adamw_entry;
 int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dtype, int out16_dtype, double lr,
                       double beta1, double beta2, double eps, double weight_decay, int64_t step,
-                      const float* grad_scale, int flags, void* stream);
+                      const float* grad_scale, int flags, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Measurement hook: arms a pair of HIP events (hipEvent_t, created with timing
  * enabled) for the calling thread.  The next kernel this thread launches

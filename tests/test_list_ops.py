@@ -1,8 +1,6 @@
 """The list passes without a GPU: what the C entry points refuse before they touch the device, what the Python side
 refuses, and the C++ pass over tensor lists against the Python checks it short-cuts."""
 
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -12,7 +10,7 @@ from yafsdp_amd import _native
 tl = pytest.importorskip("yafsdp_amd._tensorlist")
 OK, INVALID, DTYPE, MISALIGNED, TOO_LARGE, OVERLAP = 0, -1, -2, -3, -6, -9
 F32, BF16, F16 = 0, 1, 2
-WS = _native.LIST_WORKSPACE_BYTES
+WS = _native.lib.yafsdp_list_workspace_bytes(1)
 
 
 def _entries(*rows):
@@ -29,6 +27,10 @@ def _norm(entries, norm=2, workspace=0x10000, ws_bytes=WS, out=0x20000, clip=Fal
     return fn(buf, count if n is None else n, norm, 1.0, workspace, ws_bytes, out, None)
 
 
+def _scale(entries, coef=0x20000, workspace=0x10000, ws_bytes=WS):
+    return _native.lib.yafsdp_list_scale(*entries, coef, workspace, ws_bytes, None)
+
+
 # every refused call names addresses that are never read: the checks come before the first launch
 @pytest.mark.parametrize("clip", [False, True])
 def test_norm_and_clip_refusals(clip):
@@ -37,9 +39,11 @@ def test_norm_and_clip_refusals(clip):
     assert _norm(one, workspace=None, clip=clip) == INVALID
     assert _norm(one, ws_bytes=WS - 1, clip=clip) == INVALID
     assert _norm(one, out=None, clip=clip) == INVALID
-    assert _norm(one, workspace=0x10004, clip=clip) == MISALIGNED
+    assert _norm(one, workspace=0x10008, clip=clip) == MISALIGNED
     assert _norm(one, out=0x20002, clip=clip) == MISALIGNED
     assert _norm(one, n=-1, clip=clip) == INVALID
+    many = _entries(*[(0x100000 + 0x100 * i, 4, F32) for i in range(241)])
+    assert _norm(many, clip=clip) == INVALID  # a longer list needs a larger workspace
     assert _norm((None, 1), clip=clip) == INVALID
     assert _norm(_entries((0x1000, 4, 3)), clip=clip) == DTYPE
     assert _norm(_entries((0x1000, 4, -1)), clip=clip) == DTYPE
@@ -60,26 +64,26 @@ def test_norm_and_clip_refusals(clip):
 ])
 def test_writes_to_shared_memory_are_refused(call, rows):
     e = _entries(*rows)
-    rc = _norm(e, clip=True) if call == "clip" else _native.lib.yafsdp_list_scale(*e, 0x20000, None)
+    rc = _norm(e, clip=True) if call == "clip" else _scale(e)
     assert rc == OVERLAP
     assert "share memory" in _native.error_string(rc)
 
 
 def test_scale_refusals_and_empty_list():
-    L = _native.lib
     one = _entries((0x1000, 4, F32))
-    assert L.yafsdp_list_scale(*one, None, None) == INVALID
-    assert L.yafsdp_list_scale(*one, 0x20001, None) == MISALIGNED
-    assert L.yafsdp_list_scale(*_entries((0x1000, 4, 9)), 0x20000, None) == DTYPE
-    assert L.yafsdp_list_scale(*_entries((0x1002, 4, F32)), 0x20000, None) == MISALIGNED
-    assert L.yafsdp_list_scale(None, 0, 0x20000, None) == OK
-    assert L.yafsdp_list_scale(*_entries((0, 0, F32), (0x1001, 0, BF16)), 0x20000, None) == OK  # empty tensors
+    assert _scale(one, coef=None) == INVALID and _scale(one, coef=0x20001) == MISALIGNED
+    assert _scale(one, workspace=None) == INVALID and _scale(one, workspace=0x10008) == MISALIGNED
+    assert _scale(one, ws_bytes=WS - 1) == INVALID
+    assert _scale(_entries((0x1000, 4, 9))) == DTYPE
+    assert _scale(_entries((0x1002, 4, F32))) == MISALIGNED
+    assert _scale((None, 0)) == OK
+    assert _scale(_entries((0, 0, F32), (0x1001, 0, BF16))) == OK  # empty tensors
 
 
-def _adamw(entries, grad=F32, out=F32, step=1, scale=None, flags=1, n=None):
+def _adamw(entries, grad=F32, out=F32, step=1, scale=None, flags=1, n=None, workspace=None, ws_bytes=0):
     buf, count = entries
     return _native.lib.yafsdp_list_adamw(buf, count if n is None else n, grad, out, 1e-3, 0.9, 0.95, 1e-8, 0.1, step,
-                                         scale, flags, None)
+                                         scale, flags, workspace, ws_bytes, None)
 
 
 def test_adamw_refusals():
@@ -98,6 +102,10 @@ def test_adamw_refusals():
     assert _adamw(_adam((*row[:4], 0x5001, 8)), out=BF16) == MISALIGNED
     assert _adamw(_adam((0x1000, 0x2001, 0x3000, 0x4000, 0, 8)), grad=BF16) == MISALIGNED
     assert _adamw(_adam((0, 0, 0, 0, 0, 0))) == OK and _adamw((None, 0)) == OK
+    many = _adam(*[tuple(x + 0x100000 * i for x in row[:5]) + (8,) for i in range(81)])
+    need = _native.lib.yafsdp_list_adamw_workspace_bytes(81)
+    assert _adamw(many) == INVALID and _adamw(many, workspace=0x10000, ws_bytes=need - 1) == INVALID
+    assert _adamw(many, workspace=0x10008, ws_bytes=need) == MISALIGNED
     ZERO = _native.ADAM_ZERO_GRAD
     far = (0x11000, 0x12000, 0x13000, 0x14000, 0x15000, 8)
     assert _adamw(_adam(row, (0x1000, *far[1:]))) == OVERLAP              # the same parameter twice
@@ -205,13 +213,24 @@ def test_bump_versions_matches_torch():
     before = (base._version, b._version)
     tl.bump_versions([a, None, b])
     assert (base._version, b._version) == (before[0] + 1, before[1] + 1)  # a view shares its base's counter
+    tl.bump_versions([a, b], [None, 1])
+    assert (base._version, b._version) == (before[0] + 1, before[1] + 2)
     with torch.inference_mode():
         c = torch.zeros(2)
     tl.bump_versions([c])  # has none
     with pytest.raises(TypeError):
         tl.bump_versions([1])
+    with pytest.raises(TypeError):
+        tl.bump_versions([b], [])
 
 
-def test_workspace_is_a_constant():
-    assert WS == _native.lib.yafsdp_list_workspace_bytes() and WS % 8 == 0
-    assert isinstance(_native.lib.yafsdp_list_workspace_bytes(), int) and ctypes.sizeof(ctypes.c_size_t) == 8
+def test_workspace_sizes():
+    """Partial sums, and behind them (AdamW: alone) lists that the kernel arguments do not hold: 4 (12) words per entry in
+    whole pieces of 960."""
+    norm, adamw = _native.lib.yafsdp_list_workspace_bytes, _native.lib.yafsdp_list_adamw_workspace_bytes
+    assert norm(0) == norm(240) == 1024 * 8
+    for n in (241, 480, 481, 5000):
+        assert norm(n) == norm(0) + -(-4 * n // 960) * 960 * 4
+    assert adamw(0) == adamw(80) == 0
+    for n in (81, 160, 161, 3000):
+        assert adamw(n) == -(-12 * n // 960) * 960 * 4

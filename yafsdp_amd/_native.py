@@ -75,6 +75,7 @@ EXPORTED_SYMBOLS = (
     "yafsdp_flat_scale",
     "yafsdp_adamw_step",
     "yafsdp_list_workspace_bytes",
+    "yafsdp_list_adamw_workspace_bytes",
     "yafsdp_list_norm",
     "yafsdp_list_clip",
     "yafsdp_list_scale",
@@ -173,15 +174,17 @@ def _load() -> ctypes.CDLL:
     lib.yafsdp_adamw_step.restype = i32
     lib.yafsdp_adamw_step.argtypes = [vp, vp, vp, vp, vp, i32, i64, dbl, dbl, dbl, dbl, dbl, i64, vp, i32, vp]
     lib.yafsdp_list_workspace_bytes.restype = ctypes.c_size_t
-    lib.yafsdp_list_workspace_bytes.argtypes = []
+    lib.yafsdp_list_workspace_bytes.argtypes = [i64]
+    lib.yafsdp_list_adamw_workspace_bytes.restype = ctypes.c_size_t
+    lib.yafsdp_list_adamw_workspace_bytes.argtypes = [i64]
     lib.yafsdp_list_norm.restype = i32
     lib.yafsdp_list_norm.argtypes = [vp, i64, i32, dbl, vp, ctypes.c_size_t, vp, vp]
     lib.yafsdp_list_clip.restype = i32
     lib.yafsdp_list_clip.argtypes = [vp, i64, i32, dbl, vp, ctypes.c_size_t, vp, vp]
     lib.yafsdp_list_scale.restype = i32
-    lib.yafsdp_list_scale.argtypes = [vp, i64, vp, vp]
+    lib.yafsdp_list_scale.argtypes = [vp, i64, vp, vp, ctypes.c_size_t, vp]
     lib.yafsdp_list_adamw.restype = i32
-    lib.yafsdp_list_adamw.argtypes = [vp, i64, i32, i32, dbl, dbl, dbl, dbl, dbl, i64, vp, i32, vp]
+    lib.yafsdp_list_adamw.argtypes = [vp, i64, i32, i32, dbl, dbl, dbl, dbl, dbl, i64, vp, i32, vp, ctypes.c_size_t, vp]
     lib.yafsdp_time_next_launch.restype = i32
     lib.yafsdp_time_next_launch.argtypes = [vp, vp]
     lib.yafsdp_complete_next_launch.restype = i32
@@ -919,7 +922,6 @@ def adamw_step(
 
 # ---- the same passes over a list of separate tensors ---------------------------
 NORM_CODE = {1.0: 1, 2.0: 2, float("inf"): 3}
-LIST_WORKSPACE_BYTES = int(lib.yafsdp_list_workspace_bytes())
 _LIST_ENTRY = np.dtype([("data", np.uint64), ("numel", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
 _ADAMW_ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("exp_avg", np.uint64), ("exp_avg_sq", np.uint64),
                          ("out16", np.uint64), ("numel", np.int64)])
@@ -993,11 +995,12 @@ class TensorList:
         _bump_versions(self.tensors)
 
 
-def _bump_versions(tensors) -> None:
+def _bump_versions(tensors, where=None) -> None:
     if _tensorlist is not None:
-        _tensorlist.bump_versions(tensors)
-    else:
-        torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
+        _tensorlist.bump_versions(tensors, where)
+        return
+    live = [t for t, w in zip(tensors, tensors if where is None else where) if t is not None and w is not None]
+    torch.autograd.graph.increment_version([t for t in live if not t.is_inference()])
 
 
 def norm_code(norm_type) -> int:
@@ -1007,38 +1010,32 @@ def norm_code(norm_type) -> int:
         raise NotImplementedError(f"only the 1-, 2- and infinity-norm are implemented, got {norm_type}") from None
 
 
-def _check_norm_out(lst: TensorList, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
-    _flat_arg(norm_and_coef, "norm_and_coef"), _flat_arg(workspace, "workspace")
-    if norm_and_coef.dtype != torch.float32 or norm_and_coef.numel() < 2:
-        raise TypeError("norm_and_coef must be float32 with two elements")
-    if norm_and_coef.device != lst.device or workspace.device != lst.device:
-        raise RuntimeError("the tensors, norm_and_coef and workspace must live on one device")
-
-
-def list_workspace(device: torch.device) -> torch.Tensor:
-    """Scratch of ``list_norm`` / ``list_clip``; reusable across calls that do not overlap."""
-    return torch.empty(LIST_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
-
-
-def _list_norm(fn, name, lst, norm_type, max_norm, norm_and_coef, workspace) -> None:
+def _list_norm(fn, name: str, lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
     code = norm_code(norm_type)
-    _check_norm_out(lst, norm_and_coef, workspace)
+    norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
+    workspace, nbytes = _list_workspace(lst)
     with _on(lst.device):
         _check(
-            fn(lst.entries, lst.count, code, float(max_norm), workspace.data_ptr(),
-               workspace.numel() * workspace.element_size(), norm_and_coef.data_ptr(), _stream(norm_and_coef)),
+            fn(lst.entries, lst.count, code, float(max_norm), workspace.data_ptr(), nbytes, norm_and_coef.data_ptr(),
+               _stream(norm_and_coef)),
             name,
         )
+    return norm_and_coef
 
 
-def list_norm(lst: TensorList, norm_type, max_norm: float, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
-    """``{norm, clip coefficient}`` (float32) over every element of the list; ``norm_type`` 1, 2 or infinity."""
-    _list_norm(lib.yafsdp_list_norm, "yafsdp_list_norm", lst, norm_type, max_norm, norm_and_coef, workspace)
+def _list_workspace(lst: TensorList) -> "tuple[torch.Tensor, int]":
+    nbytes = lib.yafsdp_list_workspace_bytes(lst.count)
+    return torch.empty(nbytes, dtype=torch.uint8, device=lst.device), nbytes
 
 
-def list_clip(lst: TensorList, norm_type, max_norm: float, norm_and_coef: torch.Tensor, workspace: torch.Tensor) -> None:
+def list_norm(lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
+    """``[norm, clip coefficient]`` (float32) over every element of the list; ``norm_type`` 1, 2 or infinity."""
+    return _list_norm(lib.yafsdp_list_norm, "yafsdp_list_norm", lst, norm_type, max_norm)
+
+
+def list_clip(lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
     """``list_norm``, then every element times the coefficient, in place."""
-    _list_norm(lib.yafsdp_list_clip, "yafsdp_list_clip", lst, norm_type, max_norm, norm_and_coef, workspace)
+    return _list_norm(lib.yafsdp_list_clip, "yafsdp_list_clip", lst, norm_type, max_norm)
 
 
 def list_scale(lst: TensorList, coef: torch.Tensor) -> None:
@@ -1046,8 +1043,12 @@ def list_scale(lst: TensorList, coef: torch.Tensor) -> None:
     _flat_arg(coef, "coef")
     if coef.dtype != torch.float32 or coef.numel() != 1 or coef.device != lst.device:
         raise TypeError("coef must be a one-element float32 tensor on the list's device")
+    workspace, nbytes = _list_workspace(lst)
     with _on(lst.device):
-        _check(lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), _stream(coef)), "yafsdp_list_scale")
+        _check(
+            lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), workspace.data_ptr(), nbytes, _stream(coef)),
+            "yafsdp_list_scale",
+        )
 
 
 class AdamwList:
@@ -1110,10 +1111,10 @@ class AdamwList:
     def bump_versions(self, zero_grad: bool) -> None:
         """Of everything the step writes: the positions with a gradient of every list but the gradients (of those too
         where the step zero-fills them)."""
-        live = [g is not None for g in self.lists[1]]
-        for k, ts in enumerate(self.lists):
-            if ts is not None and (k != 1 or zero_grad):
-                _bump_versions(ts if all(live) else [t for t, on in zip(ts, live) if on])
+        params, grads, exp_avgs, exp_avg_sqs, outs16 = self.lists
+        for ts in (params, grads if zero_grad else None, exp_avgs, exp_avg_sqs, outs16):
+            if ts is not None:
+                _bump_versions(ts, grads)
 
 
 def list_adamw(
@@ -1129,12 +1130,14 @@ def list_adamw(
             raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
         gs_ptr = grad_scale.data_ptr()
     flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
+    need = lib.yafsdp_list_adamw_workspace_bytes(lst.count)
+    workspace = torch.empty(need, dtype=torch.uint8, device=lst.device) if need else None
     with _on(lst.device):
         stream = _raw_current_stream(lst.device.index) if _raw_current_stream is not None else (
             torch.cuda.current_stream(lst.device).cuda_stream)
         code = lib.yafsdp_list_adamw(
             lst.entries, lst.count, lst.grad_code, lst.out_code, float(lr), float(beta1), float(beta2), float(eps),
-            float(weight_decay), int(step), gs_ptr, flags, stream,
+            float(weight_decay), int(step), gs_ptr, flags, workspace.data_ptr() if need else None, need, stream,
         )
     if code == ERR_OVERLAP and allow_overlap:
         return False

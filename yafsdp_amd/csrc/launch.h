@@ -125,14 +125,27 @@ hipError_t launch_clip_coef(const double* sumsq, float max_norm, float* norm_and
 hipError_t launch_adamw(int out_dt, float* p, float* g, float* m, float* v, void* out16, int64_t n, int head,
                         const AdamScalars& s, const float* grad_scale, int grid, hipStream_t stream);
 
-// passes over a list of tensors (list.hip)
+// passes over a list of tensors (list.hip); META is ListArgs / ListAdamArgs (in the kernel arguments) or ListRef /
+// ListAdamRef (in the workspace, written by launch_list_stage), explicitly instantiated there
+hipError_t launch_list_stage(const ListStageArgs& a, uint32_t* dst, hipStream_t stream);
 // partials[0:grid] = per-workgroup shares of the norm (LIST_NORM_*)
-hipError_t launch_list_norm(int norm, const ListArgs& a, double* partials, int grid, hipStream_t stream);
+template <class META>
+hipError_t launch_list_norm(int norm, const META& a, double* partials, int grid, hipStream_t stream);
 hipError_t launch_list_finish(int norm, const double* partials, int count, float max_norm, float* norm_and_coef,
                               hipStream_t stream);
-hipError_t launch_list_scale(const ListArgs& a, const float* coef, int grid, hipStream_t stream);
+// norm, coefficient and (clip) the scaling by one workgroup
+hipError_t launch_list_small(int norm, bool clip, const ListArgs& a, float max_norm, float* norm_and_coef,
+                             hipStream_t stream);
+// launch_list_finish and the scaling by a grid that loops over the tiles
+template <class META>
+hipError_t launch_list_clip(int norm, const META& a, const double* partials, int count, float max_norm,
+                            float* norm_and_coef, int grid, hipStream_t stream);
+// one wave per tile; nothing where *coef is 1
+template <class META>
+hipError_t launch_list_scale(const META& a, const float* coef, int grid, hipStream_t stream);
 // out_dt F32: no 16-bit copy of the parameters
-hipError_t launch_list_adamw(int grad_dt, int out_dt, const ListAdamArgs& a, const AdamScalars& s,
-                             const float* grad_scale, int grid, hipStream_t stream);
+template <class META>
+hipError_t launch_list_adamw(int grad_dt, int out_dt, const META& a, const AdamScalars& s, const float* grad_scale,
+                             int grid, hipStream_t stream);
 
 }  // namespace yafsdp

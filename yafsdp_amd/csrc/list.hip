@@ -4,56 +4,87 @@
 
 namespace yafsdp {
 
-hipError_t launch_list_norm(int norm, const ListArgs& a, double* partials, int grid, hipStream_t stream) {
+namespace {
+
+// f(integral constant of the norm)
+template <int N>
+struct norm_t { static constexpr int value = N; };
+template <class F>
+hipError_t by_norm(int norm, F f) {
   switch (norm) {
-    case LIST_NORM_1:
-      return launch_kernel(list_norm_kernel<LIST_NORM_1, kListBlock>, grid, kListBlock, stream, a, partials);
-    case LIST_NORM_2:
-      return launch_kernel(list_norm_kernel<LIST_NORM_2, kListBlock>, grid, kListBlock, stream, a, partials);
-    case LIST_NORM_INF:
-      return launch_kernel(list_norm_kernel<LIST_NORM_INF, kListBlock>, grid, kListBlock, stream, a, partials);
+    case LIST_NORM_1: return f(norm_t<LIST_NORM_1>());
+    case LIST_NORM_2: return f(norm_t<LIST_NORM_2>());
+    case LIST_NORM_INF: return f(norm_t<LIST_NORM_INF>());
     default: return hipErrorInvalidValue;
   }
+}
+
+}  // namespace
+
+hipError_t launch_list_stage(const ListStageArgs& a, uint32_t* dst, hipStream_t stream) {
+  return launch_kernel(list_stage_kernel, 1, kListStageWords / 4, stream, a, reinterpret_cast<u32x4*>(dst));
+}
+
+template <class META>
+hipError_t launch_list_norm(int norm, const META& a, double* partials, int grid, hipStream_t stream) {
+  return by_norm(norm, [&](auto n) {
+    return launch_kernel(list_norm_kernel<decltype(n)::value, META, kListNormBlock>, grid, kListNormBlock, stream, a,
+                         partials);
+  });
 }
 
 hipError_t launch_list_finish(int norm, const double* partials, int count, float max_norm, float* norm_and_coef,
                               hipStream_t stream) {
-  switch (norm) {
-    case LIST_NORM_1:
-      return launch_kernel(list_finish_kernel<LIST_NORM_1, 1024>, 1, 1024, stream, partials, count, max_norm,
-                           norm_and_coef);
-    case LIST_NORM_2:
-      return launch_kernel(list_finish_kernel<LIST_NORM_2, 1024>, 1, 1024, stream, partials, count, max_norm,
-                           norm_and_coef);
-    case LIST_NORM_INF:
-      return launch_kernel(list_finish_kernel<LIST_NORM_INF, 1024>, 1, 1024, stream, partials, count, max_norm,
-                           norm_and_coef);
-    default: return hipErrorInvalidValue;
-  }
+  return by_norm(norm, [&](auto n) {
+    return launch_kernel(list_finish_kernel<decltype(n)::value, 1024>, 1, 1024, stream, partials, count, max_norm,
+                         norm_and_coef);
+  });
 }
 
-hipError_t launch_list_scale(const ListArgs& a, const float* coef, int grid, hipStream_t stream) {
-  return launch_kernel(list_scale_kernel<kListBlock>, grid, kListBlock, stream, a, coef);
+hipError_t launch_list_small(int norm, bool clip, const ListArgs& a, float max_norm, float* norm_and_coef,
+                             hipStream_t stream) {
+  return by_norm(norm, [&](auto n) {
+    if (clip)
+      return launch_kernel(list_small_kernel<decltype(n)::value, true, kListSmallBlock>, 1, kListSmallBlock, stream, a,
+                           max_norm, norm_and_coef);
+    return launch_kernel(list_small_kernel<decltype(n)::value, false, kListSmallBlock>, 1, kListSmallBlock, stream, a,
+                         max_norm, norm_and_coef);
+  });
+}
+
+template <class META>
+hipError_t launch_list_clip(int norm, const META& a, const double* partials, int count, float max_norm,
+                            float* norm_and_coef, int grid, hipStream_t stream) {
+  return by_norm(norm, [&](auto n) {
+    return launch_kernel(list_clip_kernel<decltype(n)::value, META, kListClipBlock>, grid, kListClipBlock, stream, a,
+                         partials, count, max_norm, norm_and_coef);
+  });
+}
+
+template <class META>
+hipError_t launch_list_scale(const META& a, const float* coef, int grid, hipStream_t stream) {
+  return launch_kernel(list_scale_kernel<META, kListScaleBlock>, grid, kListScaleBlock, stream, a, coef);
 }
 
 namespace {
-template <class G>
-hipError_t adamw_by_out(int out_dt, const ListAdamArgs& a, const AdamScalars& s, const float* grad_scale, int grid,
+template <class G, class META>
+hipError_t adamw_by_out(int out_dt, const META& a, const AdamScalars& s, const float* grad_scale, int grid,
                         hipStream_t stream) {
   switch (out_dt) {
     case DT_F32:
-      return launch_kernel(list_adamw_kernel<G, F32, kListBlock>, grid, kListBlock, stream, a, s, grad_scale);
+      return launch_kernel(list_adamw_kernel<G, F32, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
     case DT_BF16:
-      return launch_kernel(list_adamw_kernel<G, BF16, kListBlock>, grid, kListBlock, stream, a, s, grad_scale);
+      return launch_kernel(list_adamw_kernel<G, BF16, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
     case DT_F16:
-      return launch_kernel(list_adamw_kernel<G, F16, kListBlock>, grid, kListBlock, stream, a, s, grad_scale);
+      return launch_kernel(list_adamw_kernel<G, F16, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
     default: return hipErrorInvalidValue;
   }
 }
 }  // namespace
 
-hipError_t launch_list_adamw(int grad_dt, int out_dt, const ListAdamArgs& a, const AdamScalars& s,
-                             const float* grad_scale, int grid, hipStream_t stream) {
+template <class META>
+hipError_t launch_list_adamw(int grad_dt, int out_dt, const META& a, const AdamScalars& s, const float* grad_scale,
+                             int grid, hipStream_t stream) {
   switch (grad_dt) {
     case DT_F32: return adamw_by_out<F32>(out_dt, a, s, grad_scale, grid, stream);
     case DT_BF16: return adamw_by_out<BF16>(out_dt, a, s, grad_scale, grid, stream);
@@ -61,5 +92,17 @@ hipError_t launch_list_adamw(int grad_dt, int out_dt, const ListAdamArgs& a, con
     default: return hipErrorInvalidValue;
   }
 }
+
+#define YAFSDP_LIST_INSTANCES(META)                                                                               \
+  template hipError_t launch_list_norm<META>(int, const META&, double*, int, hipStream_t);                        \
+  template hipError_t launch_list_clip<META>(int, const META&, const double*, int, float, float*, int, hipStream_t); \
+  template hipError_t launch_list_scale<META>(const META&, const float*, int, hipStream_t);
+YAFSDP_LIST_INSTANCES(ListArgs)
+YAFSDP_LIST_INSTANCES(ListRef)
+#undef YAFSDP_LIST_INSTANCES
+template hipError_t launch_list_adamw<ListAdamArgs>(int, int, const ListAdamArgs&, const AdamScalars&, const float*, int,
+                                                    hipStream_t);
+template hipError_t launch_list_adamw<ListAdamRef>(int, int, const ListAdamRef&, const AdamScalars&, const float*, int,
+                                                   hipStream_t);
 
 }  // namespace yafsdp

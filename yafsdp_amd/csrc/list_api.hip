@@ -1,7 +1,8 @@
 // C ABI of the list entry points: argument checks, packing of the ranges into launches.  Declarations are in
 // include/yafsdp_hip.h.
 #include <algorithm>
-#include <new>
+#include <cstring>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/yafsdp_hip.h"
@@ -75,90 +76,130 @@ int check_disjoint(const std::vector<Range>& ranges) {
   return disjoint(spans) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
 }
 
-// One launch's arguments from ranges [first, first + a.n); returns the first range of the next launch.
-int pack(const std::vector<Range>& ranges, size_t first, ListArgs& a, size_t* next) {
-  uint64_t tiles = 0;
-  size_t i = first;
-  a.n = 0;
-  for (; i < ranges.size() && a.n < kListMax; i++) {
-    const Range& r = ranges[i];
-    const uint64_t end = (r.addr & 127) + r.bytes;  // counted from the line that holds the first element
-    const uint64_t n = (end + kListTileBytes - 1) / kListTileBytes;
-    if (tiles + n > uint64_t(INT32_MAX)) {
-      if (a.n == 0) return YAFSDP_ERR_TOO_LARGE;
-      break;
-    }
-    tiles += n;
-    const uint32_t tail = uint32_t(end - (n - 1) * kListTileBytes);
-    a.r[a.n++] = ListRange{r.addr, uint32_t(tiles), tail | uint32_t(r.dtype) << 30};
-  }
-  a.n_tiles = uint32_t(tiles);
-  *next = i;
-  return YAFSDP_OK;
+// workgroups of `block` lanes, one wave per tile, at most `cap`
+int grid_of(uint32_t n_tiles, int block, int64_t cap) {
+  const int per = block / 64;
+  return int(std::min((int64_t(n_tiles) + per - 1) / per, cap));
 }
 
-int grid_of(uint32_t n_tiles, int cap) {
-  const int per = kListBlock / 64;
-  const int64_t g = (int64_t(n_tiles) + per - 1) / per;
-  return int(g < cap ? g : cap);
+constexpr size_t kPartialBytes = size_t(kListNormGrid) * sizeof(double);
+constexpr size_t kAdamRecordWords = sizeof(ListAdamRange) / sizeof(uint32_t);
+
+// Bytes of `words` 32-bit words in the workspace: whole pieces of kListStageWords.
+size_t staged_bytes(size_t words) {
+  return (words + kListStageWords - 1) / kListStageWords * kListStageWords * sizeof(uint32_t);
 }
 
-// The partial sums of every range into the workspace; *count receives how many.
-int norm_launches(const std::vector<Range>& ranges, int norm, double* partials, int* count, hipStream_t stream) {
-  const int64_t launches = (int64_t(ranges.size()) + kListMax - 1) / kListMax;
-  // (a launch of fewer ranges for the sake of its tile count happens beyond 8 TB only; it is refused below)
-  int64_t cap = launches > 0 ? kListMaxPartials / launches : 0;
-  if (launches > 0 && cap < 1) return YAFSDP_ERR_TOO_LARGE;
-  cap = std::min<int64_t>(cap, kListGrid);
-  *count = 0;
-  ListArgs a;
-  for (size_t i = 0; i < ranges.size();) {
-    const int rc = pack(ranges, i, a, &i);
-    if (rc != YAFSDP_OK) return rc;
-    const int grid = grid_of(a.n_tiles, int(cap));
-    if (*count + grid > kListMaxPartials) return YAFSDP_ERR_TOO_LARGE;
-    const hipError_t e = launch_list_norm(norm, a, partials + *count, grid, stream);
-    if (e != hipSuccess) return int(e);
-    *count += grid;
-  }
-  return YAFSDP_OK;
-}
-
-int scale_launches(const std::vector<Range>& ranges, const float* coef, hipStream_t stream) {
-  ListArgs a;
-  for (size_t i = 0; i < ranges.size();) {
-    const int rc = pack(ranges, i, a, &i);
-    if (rc != YAFSDP_OK) return rc;
-    const hipError_t e = launch_list_scale(a, coef, grid_of(a.n_tiles, kListGrid), stream);
+// Sends `words` to the workspace, one launch per piece.
+int stage(const std::vector<uint32_t>& words, void* dst, hipStream_t stream) {
+  ListStageArgs a{};
+  for (size_t i = 0; i < words.size(); i += kListStageWords) {
+    std::copy_n(words.data() + i, std::min(words.size() - i, size_t(kListStageWords)), a.word);
+    const hipError_t e = launch_list_stage(a, static_cast<uint32_t*>(dst) + i, stream);
     if (e != hipSuccess) return int(e);
   }
   return YAFSDP_OK;
+}
+
+// Tile bookkeeping of range k: its tiles end at tile_end, its last one holds `tail`.
+struct Tiles {
+  uint64_t count = 0;
+  bool add(uint64_t n) { return (count += n) <= uint64_t(INT32_MAX); }
+};
+
+// Where range r lies in tiles counted from the 128-byte line that holds its first element.
+bool cut(const Range& r, Tiles& tiles, uint32_t* tile_end, uint32_t* tail) {
+  const uint64_t end = (r.addr & 127) + r.bytes, n = (end + kListTileBytes - 1) / kListTileBytes;
+  if (!tiles.add(n)) return false;
+  *tile_end = uint32_t(tiles.count);
+  *tail = uint32_t(end - (n - 1) * kListTileBytes) | uint32_t(r.dtype) << 30;
+  return true;
+}
+
+int pack(const std::vector<Range>& ranges, ListArgs& a) {
+  Tiles tiles;
+  a.n = int32_t(ranges.size());
+  for (int k = 0; k < a.n; k++) {
+    if (!cut(ranges[k], tiles, &a.tile_end[k], &a.tail[k])) return YAFSDP_ERR_TOO_LARGE;
+    a.addr[k] = ranges[k].addr;
+  }
+  a.n_tiles = uint32_t(tiles.count);
+  return YAFSDP_OK;
+}
+
+// The list behind the partial sums of the workspace: addresses, then the two word arrays.
+int pack_and_stage(const std::vector<Range>& ranges, void* workspace, hipStream_t stream, ListRef& a) {
+  const size_t n = ranges.size();
+  std::vector<uint32_t> words(4 * n);
+  Tiles tiles;
+  for (size_t k = 0; k < n; k++) {
+    words[2 * k] = uint32_t(ranges[k].addr);
+    words[2 * k + 1] = uint32_t(uint64_t(ranges[k].addr) >> 32);
+    if (!cut(ranges[k], tiles, &words[2 * n + k], &words[3 * n + k])) return YAFSDP_ERR_TOO_LARGE;
+  }
+  uint32_t* base = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kPartialBytes);
+  a = ListRef{int32_t(n), uint32_t(tiles.count), base + 2 * n, base + 3 * n, reinterpret_cast<const uint64_t*>(base)};
+  return stage(words, base, stream);
+}
+
+// f(meta) with the list in the kernel arguments or, where it is too long for them, in the workspace
+template <class F>
+int with_list(const std::vector<Range>& ranges, void* workspace, hipStream_t stream, F f) {
+  if (ranges.size() <= size_t(kListMax)) {
+    ListArgs a;
+    const int rc = pack(ranges, a);
+    return rc != YAFSDP_OK ? rc : f(a);
+  }
+  ListRef a;
+  const int rc = pack_and_stage(ranges, workspace, stream, a);
+  return rc != YAFSDP_OK ? rc : f(a);
+}
+
+template <class META>
+int norm_or_clip_launches(const META& a, int norm, float max_norm, double* partials, float* norm_and_coef, bool clip,
+                          hipStream_t stream) {
+  const bool long_ranges = a.n_tiles / uint32_t(a.n) >= uint32_t(kListNormLongRange);
+  const int count = grid_of(a.n_tiles, kListNormBlock, long_ranges ? kListNormLongGrid : kListNormGrid);
+  hipError_t e = launch_list_norm(norm, a, partials, count, stream);
+  if (e != hipSuccess) return int(e);
+  if (clip && a.n_tiles <= uint32_t(kListClipTiles))
+    return int(launch_list_clip(norm, a, partials, count, max_norm, norm_and_coef,
+                                grid_of(a.n_tiles, kListClipBlock, kListClipGrid), stream));
+  e = launch_list_finish(norm, partials, count, max_norm, norm_and_coef, stream);
+  if (e != hipSuccess || !clip) return int(e);
+  return int(launch_list_scale(a, norm_and_coef + 1, grid_of(a.n_tiles, kListScaleBlock, INT32_MAX), stream));
 }
 
 int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
                  size_t workspace_bytes, float* norm_and_coef, hipStream_t stream, bool clip) {
   if (norm != LIST_NORM_1 && norm != LIST_NORM_2 && norm != LIST_NORM_INF) return YAFSDP_ERR_INVALID_ARGUMENT;
-  if (workspace == nullptr || norm_and_coef == nullptr || workspace_bytes < yafsdp_list_workspace_bytes())
+  if (n < 0 || workspace == nullptr || norm_and_coef == nullptr || workspace_bytes < yafsdp_list_workspace_bytes(n))
     return YAFSDP_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(workspace, 8) || !aligned_to(norm_and_coef, 4)) return YAFSDP_ERR_MISALIGNED;
+  if (!aligned_to(workspace, 16) || !aligned_to(norm_and_coef, 4)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
   if (rc == YAFSDP_OK && clip) rc = check_disjoint(ranges);
   if (rc != YAFSDP_OK) return rc;
-  double* partials = static_cast<double*>(workspace);
-  int count = 0;
-  rc = norm_launches(ranges, norm, partials, &count, stream);
-  if (rc != YAFSDP_OK) return rc;
-  const hipError_t e = launch_list_finish(norm, partials, count, static_cast<float>(max_norm), norm_and_coef, stream);
-  if (e != hipSuccess) return int(e);
-  return clip ? scale_launches(ranges, norm_and_coef + 1, stream) : YAFSDP_OK;
+  return with_list(ranges, workspace, stream, [&](const auto& a) {
+    if constexpr (std::is_same<std::decay_t<decltype(a)>, ListArgs>::value)
+      if (a.n_tiles <= uint32_t(kListSmallTiles))
+        return int(launch_list_small(norm, clip, a, static_cast<float>(max_norm), norm_and_coef, stream));
+    return norm_or_clip_launches(a, norm, static_cast<float>(max_norm), static_cast<double*>(workspace), norm_and_coef,
+                                 clip, stream);
+  });
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t yafsdp_list_workspace_bytes(void) { return size_t(kListMaxPartials) * sizeof(double); }
+size_t yafsdp_list_workspace_bytes(int64_t n) {
+  return kPartialBytes + (n > kListMax ? staged_bytes(size_t(n) * 4) : 0);
+}
+
+size_t yafsdp_list_adamw_workspace_bytes(int64_t n) {
+  return n > kListAdamMax ? staged_bytes(size_t(n) * (kAdamRecordWords + 2)) : 0;
+}
 
 int yafsdp_list_norm(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
                      size_t workspace_bytes, float* norm_and_coef, void* stream) try {
@@ -176,22 +217,32 @@ int yafsdp_list_clip(const yafsdp_list_entry* entries, int64_t n, int norm, doub
   return YAFSDP_ERR_OUT_OF_MEMORY;
 }
 
-int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* stream) try {
-  if (coef == nullptr) return YAFSDP_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(coef, 4)) return YAFSDP_ERR_MISALIGNED;
+int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* workspace,
+                      size_t workspace_bytes, void* stream_) try {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (n < 0 || coef == nullptr || workspace == nullptr || workspace_bytes < yafsdp_list_workspace_bytes(n))
+    return YAFSDP_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(coef, 4) || !aligned_to(workspace, 16)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
   if (rc == YAFSDP_OK) rc = check_disjoint(ranges);
-  if (rc != YAFSDP_OK) return rc;
-  return scale_launches(ranges, coef, static_cast<hipStream_t>(stream));
+  if (rc != YAFSDP_OK || ranges.empty()) return rc;
+  return with_list(ranges, workspace, stream, [&](const auto& a) {
+    return int(launch_list_scale(a, coef, grid_of(a.n_tiles, kListScaleBlock, INT32_MAX), stream));
+  });
 } catch (...) {
   return YAFSDP_ERR_OUT_OF_MEMORY;
 }
 
 int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dtype, int out16_dtype, double lr,
                       double beta1, double beta2, double eps, double weight_decay, int64_t step,
-                      const float* grad_scale, int flags, void* stream) try {
+                      const float* grad_scale, int flags, void* workspace, size_t workspace_bytes,
+                      void* stream_) try {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
   if (n < 0 || step < 1 || (n > 0 && entries == nullptr)) return YAFSDP_ERR_INVALID_ARGUMENT;
+  const size_t need = yafsdp_list_adamw_workspace_bytes(n);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return YAFSDP_ERR_INVALID_ARGUMENT;
+  if (need > 0 && !aligned_to(workspace, 16)) return YAFSDP_ERR_MISALIGNED;
   // out16_dtype F32: no 16-bit copy
   if (!valid_dtype(grad_dtype) || !valid_dtype(out16_dtype)) return YAFSDP_ERR_UNSUPPORTED_DTYPE;
   if (grad_scale != nullptr && !aligned_to(grad_scale, 4)) return YAFSDP_ERR_MISALIGNED;
@@ -239,29 +290,46 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
                                      [](uintptr_t lo, const Span& s) { return lo < s.hi; });
     if (it != written.end() && it->lo < g.hi) return YAFSDP_ERR_OVERLAP;
   }
+  if (ranges.empty()) return YAFSDP_OK;
   const AdamScalars s = adam_scalars(lr, beta1, beta2, eps, weight_decay, step, flags);
-  ListAdamArgs a;
-  for (size_t i = 0; i < ranges.size();) {
-    uint64_t tiles = 0;
-    a.n = 0;
-    for (; i < ranges.size() && a.n < kListAdamMax; i++) {
-      const AdamRange& r = ranges[i];
-      const uint64_t k = (r.numel + kListAdamTile - 1) / kListAdamTile;
-      if (tiles + k > uint64_t(INT32_MAX)) {
-        if (a.n == 0) return YAFSDP_ERR_TOO_LARGE;
-        break;
-      }
-      tiles += k;
-      a.r[a.n++] = ListAdamRange{r.p, r.g, r.m, r.v, r.out, uint32_t(tiles),
-                                 uint32_t(r.numel - (k - 1) * kListAdamTile)};
-    }
-    a.n_tiles = uint32_t(tiles);
-    const int64_t grid = (int64_t(tiles) + kListBlock / 64 - 1) / (kListBlock / 64);
-    const hipError_t e = launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, int(grid),
-                                           static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return int(e);
+  const size_t k = ranges.size();
+  std::vector<uint32_t> tile_end(k), tail(k);
+  Tiles tiles;
+  for (size_t i = 0; i < k; i++) {
+    const uint64_t end = (ranges[i].p & 255) / 4 + ranges[i].numel, t = (end + kListAdamTile - 1) / kListAdamTile;
+    if (!tiles.add(t)) return YAFSDP_ERR_TOO_LARGE;
+    tile_end[i] = uint32_t(tiles.count);
+    tail[i] = uint32_t(end - (t - 1) * kListAdamTile);
   }
-  return YAFSDP_OK;
+  const uint32_t n_tiles = uint32_t(tiles.count);
+  const int grid = grid_of(n_tiles, kListAdamBlock, INT32_MAX);
+  const auto record = [&](size_t i) {
+    return ListAdamRange{ranges[i].p, ranges[i].g, ranges[i].m, ranges[i].v, ranges[i].out};
+  };
+  if (k <= size_t(kListAdamMax)) {
+    ListAdamArgs a;
+    a.n = int32_t(k);
+    a.n_tiles = n_tiles;
+    for (size_t i = 0; i < k; i++) {
+      a.r[i] = record(i);
+      a.tile_end[i] = tile_end[i];
+      a.tail[i] = tail[i];
+    }
+    return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, grid, stream));
+  }
+  std::vector<uint32_t> words((kAdamRecordWords + 2) * k);
+  for (size_t i = 0; i < k; i++) {
+    const ListAdamRange r = record(i);
+    std::memcpy(&words[kAdamRecordWords * i], &r, sizeof(r));
+  }
+  std::copy(tile_end.begin(), tile_end.end(), words.begin() + kAdamRecordWords * k);
+  std::copy(tail.begin(), tail.end(), words.begin() + (kAdamRecordWords + 1) * k);
+  const int rc = stage(words, workspace, stream);
+  if (rc != YAFSDP_OK) return rc;
+  const uint32_t* base = static_cast<const uint32_t*>(workspace);
+  const ListAdamRef a{int32_t(k), n_tiles, base + kAdamRecordWords * k, base + (kAdamRecordWords + 1) * k,
+                      static_cast<const ListAdamRange*>(workspace)};
+  return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, grid, stream));
 } catch (...) {
   return YAFSDP_ERR_OUT_OF_MEMORY;
 }

@@ -1,53 +1,80 @@
-// What a list launch carries in its kernel arguments: the ranges of memory its waves walk, cut into tiles.  Shared by
-// the host packing (list_api.hip) and the kernels (list_kernels.hip.h); plain structs, no HIP types.
+// What a list launch works from: the ranges of memory its waves walk, cut into tiles.  Shared by the host packing
+// (list_api.hip) and the kernels (list_kernels.hip.h); plain structs, no HIP types.
 //
-// The ranges travel by value (at most 4 KiB of kernel arguments per launch), so a call needs no device-side table, no
-// staging copy and no state that outlives it: two calls at once, on any streams, share nothing, and a captured graph
-// holds its own copy.  A list of more ranges than fit becomes several launches.
+// Up to kListMax (kListAdamMax) ranges travel by value in the kernel arguments (at most 4 KiB per launch).  Longer lists
+// are first written to the caller's workspace by stage kernels, which carry them in THEIR arguments, and the one launch
+// that does the work reads them from there.  Either way a call needs no table that outlives it, no host-to-device copy
+// and no pinned memory: two calls at once, on any streams, share nothing, and a captured graph holds its own list.
 #pragma once
 #include <stdint.h>
 
 namespace yafsdp {
 
 // ---- norm / scale: one wave per tile of 4 KiB ---------------------------------------------------------
-constexpr int kListTileBytes = 4096;
-constexpr int kListMax = 240;  // ranges per launch: 16 bytes each
-
-struct ListRange {
-  uint64_t addr;      // first element
-  uint32_t tile_end;  // tiles of this launch up to and including this range's
-  uint32_t tail;      // bits 0-12: end of the range inside its last tile (1 .. 4096 bytes); bits 30-31: dtype
-};
 // A range's tiles start at the 128-byte line that holds its first element, so every 16-byte access is aligned and no
 // cache line is shared by two tiles of one range.
-struct ListArgs {
-  int32_t n;         // ranges
-  uint32_t n_tiles;  // of all of them
-  ListRange r[kListMax];
-};
-static_assert(sizeof(ListArgs) <= 3856, "kernel arguments hold at most 4 KiB");
+constexpr int kListTileBytes = 4096;
+constexpr int kListMax = 240;
 
-// ---- AdamW: one wave per tile of 512 elements ---------------------------------------------------------
-constexpr int kListAdamTile = 512;
-constexpr int kListAdamMax = 80;  // ranges per launch: 48 bytes each
+struct ListArgs {
+  int32_t n;                    // ranges
+  uint32_t n_tiles;             // of all of them
+  uint32_t tile_end[kListMax];  // tiles up to and including this range's
+  uint32_t tail[kListMax];      // bits 0-12: end of the range inside its last tile (1 .. 4096 bytes); bits 30-31: dtype
+  uint64_t addr[kListMax];      // first element
+};
+struct ListRef {  // the same in the workspace
+  int32_t n;
+  uint32_t n_tiles;
+  const uint32_t* tile_end;
+  const uint32_t* tail;
+  const uint64_t* addr;
+};
+
+// ---- AdamW: one wave per tile of 256 elements ---------------------------------------------------------
+// A range's tiles start at the 256-byte boundary below its first parameter (64 elements: whole lines of the 16-bit
+// arrays too).  Ranges cut from buffers of one layout have their other arrays at the matching places.
+constexpr int kListAdamTile = 256;
+constexpr int kListAdamMax = 80;
 
 struct ListAdamRange {
   uint64_t p, g, m, v, out;
-  uint32_t tile_end;
-  uint32_t tail;  // elements in the last tile (1 .. 512)
 };
 struct ListAdamArgs {
   int32_t n;
   uint32_t n_tiles;
+  uint32_t tile_end[kListAdamMax];
+  uint32_t tail[kListAdamMax];  // end of the range inside its last tile (1 .. 256)
   ListAdamRange r[kListAdamMax];
 };
-static_assert(sizeof(ListAdamArgs) <= 3856, "kernel arguments hold at most 4 KiB");
+struct ListAdamRef {
+  int32_t n;
+  uint32_t n_tiles;
+  const uint32_t* tile_end;
+  const uint32_t* tail;
+  const ListAdamRange* r;
+};
+
+// ---- staging of longer lists --------------------------------------------------------------------------
+constexpr int kListStageWords = 960;  // per launch; the workspace holds whole pieces
+struct ListStageArgs {
+  alignas(16) uint32_t word[kListStageWords];
+};
+static_assert(sizeof(ListArgs) <= 3856 && sizeof(ListAdamArgs) <= 3856 && sizeof(ListStageArgs) <= 3856,
+              "kernel arguments hold at most 4 KiB");
 
 enum : int { LIST_NORM_1 = 1, LIST_NORM_2 = 2, LIST_NORM_INF = 3 };
 
-// partial sums of one call (doubles in the caller's workspace) and workgroups of one launch
-constexpr int kListMaxPartials = 8192;
-constexpr int kListBlock = 256;
-constexpr int kListGrid = 2048;
+constexpr int kListNormBlock = 256;
+constexpr int kListNormGrid = 1024;  // = the most partial sums of one call (doubles in the caller's workspace)
+constexpr int kListNormLongGrid = 512;
+constexpr int kListNormLongRange = 1024;
+constexpr int kListSmallBlock = 1024;
+constexpr int kListSmallTiles = 128;
+constexpr int kListScaleBlock = 64;
+constexpr int kListClipBlock = 256;
+constexpr int kListClipGrid = 1024;
+constexpr int kListClipTiles = 32768;
+constexpr int kListAdamBlock = 64;
 
 }  // namespace yafsdp

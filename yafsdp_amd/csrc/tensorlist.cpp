@@ -178,14 +178,18 @@ py::object adamw_entries(py::handle params, py::handle grads, py::handle exp_avg
                         grad_code, out_code);
 }
 
-// What an in-place torch op does to its tensors' version counters (the kernels write behind autograd's back).
-void bump_versions(py::handle tensors) {
-  PyObject* seq = tensors.ptr();
-  if (!PyList_Check(seq) && !PyTuple_Check(seq)) throw py::type_error("expected a list or tuple of tensors");
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
-  PyObject** items = PySequence_Fast_ITEMS(seq);
+// What an in-place torch op does to its tensors' version counters (the kernels write behind autograd's back).  With
+// `where` (a list of the same length) only positions that are not None there.
+void bump_versions(py::handle tensors, py::handle where) {
+  PyObject* seqs[2] = {tensors.ptr(), where.is_none() ? tensors.ptr() : where.ptr()};
+  for (PyObject* s : seqs)
+    if (!PyList_Check(s) && !PyTuple_Check(s)) throw py::type_error("expected a list or tuple of tensors");
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seqs[0]);
+  if (PySequence_Fast_GET_SIZE(seqs[1]) != n) throw py::type_error("expected lists of one length");
+  PyObject** items = PySequence_Fast_ITEMS(seqs[0]);
+  PyObject** on = PySequence_Fast_ITEMS(seqs[1]);
   for (Py_ssize_t i = 0; i < n; ++i) {
-    if (items[i] == Py_None) continue;
+    if (items[i] == Py_None || on[i] == Py_None) continue;
     if (!THPVariable_Check(items[i])) throw py::type_error("expected a list or tuple of tensors");
     const at::Tensor& t = THPVariable_Unpack(items[i]);
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -200,5 +204,5 @@ PYBIND11_MODULE(_tensorlist, m) {
   m.def("all_contiguous", &all_contiguous);
   m.def("list_entries", &list_entries, "yafsdp_list_entry array of a list of tensors");
   m.def("adamw_entries", &adamw_entries, "yafsdp_adamw_entry array of parallel lists of tensors");
-  m.def("bump_versions", &bump_versions);
+  m.def("bump_versions", &bump_versions, py::arg("tensors"), py::arg("where") = py::none());
 }

@@ -297,10 +297,7 @@ def list_clip_coef(
     is 1, 2 or infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64
     and are reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls;
     the call can be captured into a HIP graph, which then reads the same addresses at every replay."""
-    lst = _native.TensorList(grads, "grads", _resolve)
-    norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
-    _native.list_norm(lst, norm_type, max_norm, norm_and_coef, _native.list_workspace(lst.device))
-    return norm_and_coef[0], norm_and_coef[1]
+    return _native.list_norm(_native.TensorList(grads, "grads", _resolve), norm_type, max_norm).unbind()
 
 
 def list_grad_norm(grads: Iterable[torch.Tensor | None], norm_type: float = 2.0) -> torch.Tensor:
@@ -315,13 +312,11 @@ def list_clip_grad_norm_(
     by the clip coefficient in binary32 and rounded to its tensor's dtype, in place; returns the total norm.  Nothing is
     written when nothing is clipped.  The tensors must not share memory."""
     lst = _native.TensorList(grads, "grads", _resolve)
-    norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
-    _native.list_clip(lst, norm_type, max_norm, norm_and_coef, _native.list_workspace(lst.device))
+    norm_and_coef = _native.list_clip(lst, norm_type, max_norm)
     lst.bump_versions()
     return norm_and_coef[0]
 
 
-@torch.no_grad()
 def list_adamw_step(
     params: Sequence[torch.Tensor],
     grads: Sequence[torch.Tensor | None],
@@ -352,7 +347,7 @@ def list_adamw_step(
     lst = _native.AdamwList(params, grads, exp_avgs, exp_avg_sqs, outs16, _resolve)
     _native.list_adamw(
         lst, lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, step=step,
-        decoupled=decoupled_weight_decay, grad_scale=None if grad_scale is None else grad_scale.view(1),
+        decoupled=decoupled_weight_decay, grad_scale=None if grad_scale is None else grad_scale.detach().view(1),
         zero_grad=zero_grad,
     )
     lst.bump_versions(zero_grad)
