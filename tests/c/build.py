@@ -37,6 +37,17 @@ def build_stage_ring_check() -> str:
     return RING_OUT
 
 
+SLOTS_OUT = os.path.join(HERE, "stage_slots_check")
+
+
+def build_stage_slots_check() -> str:
+    """Host-only check of the lists' staging slots (``yafsdp_amd/csrc/stage_slots.h``): g++, threads, no HIP."""
+    cmd = ["g++", "-O1", "-std=c++17", "-Wall", "-pthread", os.path.join(HERE, "stage_slots_check.cpp"), "-o", SLOTS_OUT]
+    subprocess.run(cmd, check=True)
+    return SLOTS_OUT
+
+
 if __name__ == "__main__":
     print(build())
     print(build_stage_ring_check())
+    print(build_stage_slots_check())

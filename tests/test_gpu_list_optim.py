@@ -476,6 +476,38 @@ def test_two_threads_at_once():
             assert_bits_equal(x, want[k], f"thread {k}")
 
 
+def test_more_long_lists_in_flight_than_staging_slots():
+    """Sixty calls whose lists go through the workspace, queued on two streams behind other work: the later ones find
+    every staging slot unread."""
+    from yafsdp_amd.optim import list_adamw_step, list_clip_coef
+
+    numels = [int(x) for x in np.random.default_rng(60).integers(1, 400, 300)]
+    gen = torch.Generator().manual_seed(60)
+    sets = []
+    for _ in range(30):
+        cpu, starts = _adam_case(numels, BF16, None, 1, 0, int(torch.randint(1 << 30, (1,), generator=gen)))
+        sets.append((cpu, {k: b.to(DEV) for k, b in cpu.items()}))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    out = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(40_000_000)
+    for i, (_, dev) in enumerate(sets):
+        with torch.cuda.stream(streams[i % 2]):
+            lists = {k: _views(b, starts, numels) for k, b in dev.items()}
+            norm, coef = list_clip_coef(lists["g"], 1e-3)
+            list_adamw_step(lists["p"], lists["g"], lists["m"], lists["v"], step=2, grad_scale=coef, **HP)
+            out.append((norm, coef))
+    torch.cuda.synchronize()
+    for (cpu, dev), (norm, coef) in zip(sets, out):
+        _assert_norm(norm, _views(cpu["g"], starts, numels), 2.0)
+        assert float(coef) == _coef32(norm.item(), 1e-3)
+        _oracle_step(cpu, starts, numels, None, False, step=2, grad_scale=float(coef), **CHP)
+        for k in "pmv":
+            assert_bits_equal(dev[k], cpu[k], k)
+
+
 def test_captured_step_replays_with_new_gradients():
     """Clip in place, then norm -> AdamW with the coefficient, captured once: two graphs alternate, eager calls and
     synchronizations in between, every replay against the same calls made eagerly on copies."""

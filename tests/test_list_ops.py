@@ -234,3 +234,19 @@ def test_workspace_sizes():
     assert adamw(0) == adamw(80) == 0
     for n in (81, 160, 161, 3000):
         assert adamw(n) == -(-12 * n // 960) * 960 * 4
+
+
+def test_staging_slots_with_a_simulated_gpu():
+    """Threads claim, fill and queue slots while another plays the GPU that reads them late and out of order between
+    queues: what it reads is what was filled, and a claim fails only while every slot is unread."""
+    import importlib.util
+    import os
+    import subprocess
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    spec = importlib.util.spec_from_file_location("c_build", os.path.join(here, "c", "build.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    out = subprocess.run([mod.build_stage_slots_check()], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout + out.stderr
+    assert "ok" in out.stdout

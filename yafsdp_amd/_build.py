@@ -17,7 +17,7 @@ SOURCES = ["api.hip", "flat.hip", "gather.hip", "scatter.hip", "optim.hip", "fan
            "list.hip", "list_api.hip"]
 HEADERS = ["elem.hip.h", "flat_kernels.hip.h", "table_kernels.hip.h", "optim_kernels.hip.h", "fan_kernels.hip.h",
            "post_sumsq_kernels.hip.h", "fused_kernels.hip.h", "list_kernels.hip.h", "list_args.h", "adam_elem.hip.h", "adam_scalars.h",
-           "launch.h", "stage_ring.h", "tuning.h"]
+           "launch.h", "stage_ring.h", "stage_slots.h", "tuning.h"]
 ARCH = "gfx950"
 
 # -ffp-contract=off: every multiply and add of the path rounds on its own, as

@@ -126,8 +126,11 @@ hipError_t launch_adamw(int out_dt, float* p, float* g, float* m, float* v, void
                         const AdamScalars& s, const float* grad_scale, int grid, hipStream_t stream);
 
 // passes over a list of tensors (list.hip); META is ListArgs / ListAdamArgs (in the kernel arguments) or ListRef /
-// ListAdamRef (in the workspace, written by launch_list_stage), explicitly instantiated there
+// ListAdamRef (in the workspace, written by launch_list_stage or launch_list_fetch), explicitly instantiated there
 hipError_t launch_list_stage(const ListStageArgs& a, uint32_t* dst, hipStream_t stream);
+// dst[0:n] = src[0:n] (16-byte vectors, src pinned), then done[0:grid] = number; grid = ceil(n / kListFetchBlock)
+hipError_t launch_list_fetch(const void* src, void* dst, uint32_t n, uint32_t* done, uint32_t number, int grid,
+                             hipStream_t stream);
 // partials[0:grid] = per-workgroup shares of the norm (LIST_NORM_*)
 template <class META>
 hipError_t launch_list_norm(int norm, const META& a, double* partials, int grid, hipStream_t stream);

@@ -25,6 +25,12 @@ hipError_t launch_list_stage(const ListStageArgs& a, uint32_t* dst, hipStream_t 
   return launch_kernel(list_stage_kernel, 1, kListStageWords / 4, stream, a, reinterpret_cast<u32x4*>(dst));
 }
 
+hipError_t launch_list_fetch(const void* src, void* dst, uint32_t n, uint32_t* done, uint32_t number, int grid,
+                             hipStream_t stream) {
+  return launch_kernel(list_fetch_kernel, grid, kListFetchBlock, stream, static_cast<const u32x4*>(src),
+                       static_cast<u32x4*>(dst), n, done, number);
+}
+
 template <class META>
 hipError_t launch_list_norm(int norm, const META& a, double* partials, int grid, hipStream_t stream) {
   return by_norm(norm, [&](auto n) {

@@ -9,6 +9,7 @@
 #include "adam_scalars.h"
 #include "launch.h"
 #include "list_args.h"
+#include "stage_slots.h"
 
 using namespace yafsdp;
 
@@ -33,15 +34,22 @@ inline bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<ui
 // more elements than any address space holds: refused before a size is computed from them
 constexpr int64_t kMaxNumel = int64_t(1) << 46;
 
-// True if no two spans share a byte.  Lists usually come in ascending order (or nearly), which costs one pass.
-bool disjoint(std::vector<Span>& s) {
-  bool ascending = true;
-  for (size_t i = 1; i < s.size() && ascending; i++) ascending = s[i - 1].hi <= s[i].lo;
-  if (ascending) return true;
-  std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+// Sorts by address; lists usually come in ascending order, which costs one pass.
+void sort_spans(std::vector<Span>& s) {
+  const auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(s.begin(), s.end(), less)) std::sort(s.begin(), s.end(), less);
+}
+// True if no two of the sorted spans share a byte.
+bool disjoint(const std::vector<Span>& s) {
   for (size_t i = 1; i < s.size(); i++)
     if (s[i - 1].hi > s[i].lo) return false;
   return true;
+}
+// Adds sorted spans to sorted spans.
+void merge_spans(std::vector<Span>& into, const std::vector<Span>& s) {
+  const size_t mid = into.size();
+  into.insert(into.end(), s.begin(), s.end());
+  std::inplace_merge(into.begin(), into.begin() + mid, into.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
 }
 
 // The list as ranges of memory: empty tensors left out, neighbours in memory of one dtype joined.
@@ -73,6 +81,7 @@ int check_disjoint(const std::vector<Range>& ranges) {
   std::vector<Span> spans;
   spans.reserve(ranges.size());
   for (const Range& r : ranges) spans.push_back(Span{r.addr, r.addr + r.bytes});
+  sort_spans(spans);
   return disjoint(spans) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
 }
 
@@ -90,8 +99,61 @@ size_t staged_bytes(size_t words) {
   return (words + kListStageWords - 1) / kListStageWords * kListStageWords * sizeof(uint32_t);
 }
 
-// Sends `words` to the workspace, one launch per piece.
+// The process's staging slots (never freed: kernels may read them until the end), or nullptr without pinned memory.
+// Call with the mutex of slots() held.
+StageSlots& slots() {
+  static StageSlots* s = new StageSlots;
+  return *s;
+}
+bool have_slots(StageSlots& s) {
+  static bool tried = false;
+  if (!tried) {
+    tried = true;
+    // an allocation is not part of anybody's graph capture
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool exchanged = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    void* block = nullptr;
+    if (hipHostMalloc(&block, StageSlots::kBlockBytes, hipHostMallocPortable | hipHostMallocMapped | hipHostMallocCoherent) ==
+        hipSuccess)
+      s.attach(block);
+    if (exchanged) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    (void)hipGetLastError();  // without pinned memory the other route serves
+  }
+  return s.attached();
+}
+
+bool capturing(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return true;
+  }
+  return status != hipStreamCaptureStatusNone;
+}
+
+// Sends `words` (a multiple of 4) to the workspace: one launch through a staging slot, or a launch per kListStageWords.
+// What a captured graph replays has to be in the graph itself, so a capture always takes the second route.
 int stage(const std::vector<uint32_t>& words, void* dst, hipStream_t stream) {
+  const size_t bytes = words.size() * sizeof(uint32_t);
+  if (!capturing(stream)) {
+    StageSlots& s = slots();
+    int slot = -1;
+    uint32_t number = 0;
+    {
+      std::lock_guard<std::mutex> lock(s.mutex);
+      if (have_slots(s)) slot = s.claim(bytes, &number);
+    }
+    if (slot >= 0) {
+      std::memcpy(s.data(slot), words.data(), bytes);
+      const hipError_t e = launch_list_fetch(s.data(slot), dst, uint32_t(bytes / 16),
+                                             reinterpret_cast<uint32_t*>(s.done(slot)), number, StageSlots::pieces(bytes),
+                                             stream);
+      if (e == hipSuccess) return YAFSDP_OK;
+      std::lock_guard<std::mutex> lock(s.mutex);
+      s.abandon(slot);
+      return int(e);
+    }
+  }
   ListStageArgs a{};
   for (size_t i = 0; i < words.size(); i += kListStageWords) {
     std::copy_n(words.data() + i, std::min(words.size() - i, size_t(kListStageWords)), a.word);
@@ -100,6 +162,7 @@ int stage(const std::vector<uint32_t>& words, void* dst, hipStream_t stream) {
   }
   return YAFSDP_OK;
 }
+static_assert(StageSlots::kPieceBytes == size_t(kListFetchBlock) * 16, "a workgroup reads a piece");
 
 // Tile bookkeeping of range k: its tiles end at tile_end, its last one holds `tail`.
 struct Tiles {
@@ -274,21 +337,23 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
     ranges.push_back(r);
   }
   // what is written shares no byte with anything else; gradients that are only read may share theirs
-  std::vector<Span> written, read;
-  for (const AdamRange& r : ranges) {
-    written.push_back(Span{r.p, r.p + 4 * r.numel});
-    (zero ? written : read).push_back(Span{r.g, r.g + gsize * r.numel});
-    written.push_back(Span{r.m, r.m + 4 * r.numel});
-    written.push_back(Span{r.v, r.v + 4 * r.numel});
-    if (has_out) written.push_back(Span{r.out, r.out + 2 * r.numel});
-  }
+  std::vector<Span> written, spans(ranges.size());
+  const auto add = [&](uintptr_t AdamRange::*member, uint64_t size, bool is_written) {
+    for (size_t i = 0; i < ranges.size(); i++)
+      spans[i] = Span{ranges[i].*member, ranges[i].*member + size * ranges[i].numel};
+    sort_spans(spans);
+    if (is_written) merge_spans(written, spans);
+  };
+  add(&AdamRange::p, 4, true);
+  add(&AdamRange::m, 4, true);
+  add(&AdamRange::v, 4, true);
+  if (has_out) add(&AdamRange::out, 2, true);
+  add(&AdamRange::g, gsize, zero);
   if (!disjoint(written)) return YAFSDP_ERR_OVERLAP;
-  std::sort(written.begin(), written.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
-  for (const Span& g : read) {
-    // the first written span that ends behind the gradient's start
-    const auto it = std::upper_bound(written.begin(), written.end(), g.lo,
-                                     [](uintptr_t lo, const Span& s) { return lo < s.hi; });
-    if (it != written.end() && it->lo < g.hi) return YAFSDP_ERR_OVERLAP;
+  size_t w = 0;
+  for (size_t i = 0; i < spans.size() && !zero; i++) {  // the gradients, sorted, against what is written
+    while (w < written.size() && written[w].hi <= spans[i].lo) w++;
+    if (w < written.size() && written[w].lo < spans[i].hi) return YAFSDP_ERR_OVERLAP;
   }
   if (ranges.empty()) return YAFSDP_OK;
   const AdamScalars s = adam_scalars(lr, beta1, beta2, eps, weight_decay, step, flags);

@@ -1,10 +1,11 @@
 // What a list launch works from: the ranges of memory its waves walk, cut into tiles.  Shared by the host packing
 // (list_api.hip) and the kernels (list_kernels.hip.h); plain structs, no HIP types.
 //
-// Up to kListMax (kListAdamMax) ranges travel by value in the kernel arguments (at most 4 KiB per launch).  Longer lists
-// are first written to the caller's workspace by stage kernels, which carry them in THEIR arguments, and the one launch
-// that does the work reads them from there.  Either way a call needs no table that outlives it, no host-to-device copy
-// and no pinned memory: two calls at once, on any streams, share nothing, and a captured graph holds its own list.
+// Up to kListMax (kListAdamMax) ranges travel by value in the kernel arguments (at most 4 KiB per launch).  A longer list
+// is first written to the caller's workspace, where the one launch that does the work reads it: by one kernel that
+// fetches it from a pinned staging slot (stage_slots.h), or, while a graph is being captured and when every slot is
+// still unread, by kernels that carry it in THEIR arguments, 3840 bytes each.  Either way no call waits for another,
+// two calls at once share nothing, and a captured graph holds its own list.
 #pragma once
 #include <stdint.h>
 
@@ -62,6 +63,8 @@ struct ListStageArgs {
 };
 static_assert(sizeof(ListArgs) <= 3856 && sizeof(ListAdamArgs) <= 3856 && sizeof(ListStageArgs) <= 3856,
               "kernel arguments hold at most 4 KiB");
+
+constexpr int kListFetchBlock = 1024;
 
 enum : int { LIST_NORM_1 = 1, LIST_NORM_2 = 2, LIST_NORM_INF = 3 };
 

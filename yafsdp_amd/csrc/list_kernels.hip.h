@@ -75,6 +75,15 @@ __global__ void __launch_bounds__(kListStageWords / 4) list_stage_kernel(ListSta
   dst[threadIdx.x] = a[threadIdx.x];
 }
 
+// The same from pinned host memory in one launch; each workgroup marks its piece as read (StageSlots).
+__global__ void __launch_bounds__(kListFetchBlock)
+list_fetch_kernel(const u32x4* src, u32x4* dst, uint32_t n, uint32_t* done, uint32_t number) {
+  const uint32_t i = blockIdx.x * kListFetchBlock + threadIdx.x;
+  if (i < n) dst[i] = src[i];
+  __syncthreads();
+  if (threadIdx.x == 0) __hip_atomic_store(done + blockIdx.x, number, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 // The ranges' addresses are integers in the list: said to be global memory here, so that the accesses need no flat ones.
 #define YAFSDP_GLOBAL_AS __attribute__((address_space(1)))
 template <class T>
