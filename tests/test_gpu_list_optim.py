@@ -337,6 +337,30 @@ def test_adamw_bits(gdtype, odtype, gap, first, zero, decoupled, scale):
             assert_bits_equal(dev[k], cpu[k], f"buffer {k} after step {step}")
 
 
+@pytest.mark.parametrize("gdtype,odtype", [(F32, None), (BF16, F16), (F16, BF16)])
+def test_adamw_of_arrays_at_different_offsets(gdtype, odtype):
+    """Nothing but the element size aligns the arrays with each other."""
+    from yafsdp_amd.optim import list_adamw_step
+
+    numels, first = [1, 5, 700, 4099, 64], {"p": 1, "g": 3, "m": 2, "v": 7, "o": 5}
+    cpu, starts = {}, {}
+    for k in ("p", "g", "m", "v") + (("o",) if odtype is not None else ()):
+        case, at = _adam_case(numels, gdtype, odtype, first[k], first[k], 12)
+        cpu[k], starts[k] = case[k], at
+    dev = {k: b.to(DEV) for k, b in cpu.items()}
+    lists = {k: _views(dev[k], starts[k], numels) for k in dev}
+    list_adamw_step(lists["p"], lists["g"], lists["m"], lists["v"], lists.get("o"), step=2, zero_grad=True, **HP)
+    for i, n in enumerate(numels):
+        part = {k: cpu[k][starts[k][i]:starts[k][i] + n] for k in cpu}
+        fresh = {k: x.clone() for k, x in part.items()}
+        cref.adamw_step(fresh["p"], part["g"].float(), fresh["m"], fresh["v"], fresh.get("o"), step=2, **CHP)
+        for k, x in fresh.items():
+            part[k].copy_(x)
+        part["g"].zero_()
+    for k in cpu:
+        assert_bits_equal(dev[k], cpu[k], k)
+
+
 @pytest.mark.parametrize("beta1,wd", [(0.3, 0.1), (0.9, 0.0), (0.0, 0.1)])
 def test_adamw_other_hyperparameters(beta1, wd):
     from yafsdp_amd.optim import list_adamw_step
@@ -584,6 +608,67 @@ def test_more_than_2_to_the_31_elements():
     assert int((big != 0).sum()) == len(at)
     del big
     torch.cuda.empty_cache()
+
+
+def test_adamw_of_more_tiles_than_one_launch_takes():
+    """2^30 elements and a few: every element against the flat pass on a copy."""
+    from yafsdp_amd import _native
+    from yafsdp_amd.optim import list_adamw_step
+
+    n = (1 << 30) + 1029
+    gen = torch.Generator(device=DEV).manual_seed(70)
+    p, g, m = (torch.randn(n, device=DEV, generator=gen).mul_(1e-2) for _ in range(3))
+    v = torch.randn(n, device=DEV, generator=gen).mul_(1e-2).square_()
+    want = [t.clone() for t in (p, m, v)]
+    list_adamw_step([p], [g], [m], [v], step=3, **HP)
+    _native.adamw_step(want[0], g, want[1], want[2], None, step=3, **CHP)
+    for a, b in zip((p, m, v), want):
+        assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+    del p, g, m, v, want, a, b
+    torch.cuda.empty_cache()
+
+
+def test_clip_of_more_tiles_than_one_launch_takes():
+    """2^22 tiles of 4 KiB and two: 17 GB of bfloat16, non-zero on both sides of every border."""
+    from yafsdp_amd.optim import list_clip_grad_norm_
+
+    n = (1 << 33) + 4099
+    big = torch.zeros(n, dtype=BF16, device=DEV)
+    at = [0, (1 << 31) + 1, (1 << 32) - 1, 1 << 32, (1 << 33) - 1, 1 << 33, (1 << 33) + 2048, n - 1]
+    for i in at:
+        big[i] = 3.0
+    norm = list_clip_grad_norm_([big], 1.0)
+    assert norm.item() == float(np.float32(math.sqrt(9.0 * len(at))))
+    want = torch.full((len(at),), 3.0, dtype=BF16)
+    cref.flat_scale(want, _coef32(norm.item(), 1.0))
+    assert_bits_equal(torch.stack([big[i] for i in at]), want, "elements on both sides of the borders")
+    assert sum(int(torch.count_nonzero(c)) for c in big.split(1 << 30)) == len(at)
+    del big
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("count", [7, 300])
+def test_without_the_native_list_helper(count, monkeypatch):
+    """The Python checks build the same entries: same bits."""
+    from yafsdp_amd import _native
+    from yafsdp_amd.optim import list_adamw_step, list_clip_grad_norm_
+
+    numels = [int(x) for x in np.random.default_rng(count).integers(0, 600, count)]
+    cpu, starts = _adam_case(numels, BF16, F16, 1, 0, 13)
+    results = []
+    for helper in (True, False):
+        if not helper:
+            monkeypatch.setattr(_native, "_tensorlist", None)
+        dev = {k: b.to(DEV) for k, b in cpu.items()}
+        lists = {k: _views(b, starts, numels) for k, b in dev.items()}
+        lists["g"][1] = None
+        norm = list_clip_grad_norm_(lists["g"], 0.01)
+        versions = [lists["p"][0]._version, dev["m"]._version]
+        list_adamw_step(lists["p"], lists["g"], lists["m"], lists["v"], lists["o"], step=2, **HP)
+        assert lists["p"][0]._version > versions[0] and dev["m"]._version > versions[1]
+        results.append([norm, *dev.values()])
+    for a, b in zip(*results):
+        assert_bits_equal(a, b, "with and without the helper")
 
 
 # -------------------------------------------------------------------------------------------- used together ----

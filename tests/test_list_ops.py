@@ -132,8 +132,14 @@ def test_lists_that_are_refused():
             fn(torch.zeros(4))
         with pytest.raises(TypeError, match="must be a tensor"):
             fn([1.0])
+        with pytest.raises(NotImplementedError, match="strided"):
+            fn([torch.zeros(3).to_sparse()])
     with pytest.raises(ValueError, match="Invalid step"):
         optim.list_adamw_step([], [], [], [], step=0)
+    for wrong in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+                  dict(lr=float("nan"))):
+        with pytest.raises(ValueError, match="Invalid"):
+            optim.list_adamw_step([], [], [], [], step=1, **wrong)
     with pytest.raises(ValueError, match="no parameter"):
         optim.list_adamw_step([torch.zeros(2)], [None], [torch.zeros(2)], [torch.zeros(2)], step=1)
     with pytest.raises(ValueError, match="exp_avgs: expected 1"):

@@ -944,6 +944,8 @@ def _is_dense(t: torch.Tensor) -> bool:
 def _list_device(t: torch.Tensor, what: str, device: torch.device | None) -> torch.device:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
+    if t.layout != torch.strided:
+        raise NotImplementedError(f"{what} must be a strided tensor, got {t.layout}")
     if t.device.type != "cuda":
         raise RuntimeError(f"{what} must live on the GPU, got {t.device}: this path has no CPU implementation")
     if device is not None and t.device != device:

@@ -145,10 +145,10 @@ hipError_t launch_list_clip(int norm, const META& a, const double* partials, int
                             float* norm_and_coef, int grid, hipStream_t stream);
 // one wave per tile; nothing where *coef is 1
 template <class META>
-hipError_t launch_list_scale(const META& a, const float* coef, int grid, hipStream_t stream);
+hipError_t launch_list_scale(const META& a, const float* coef, hipStream_t stream);
 // out_dt F32: no 16-bit copy of the parameters
 template <class META>
 hipError_t launch_list_adamw(int grad_dt, int out_dt, const META& a, const AdamScalars& s, const float* grad_scale,
-                             int grid, hipStream_t stream);
+                             hipStream_t stream);
 
 }  // namespace yafsdp

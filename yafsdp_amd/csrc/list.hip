@@ -67,22 +67,41 @@ hipError_t launch_list_clip(int norm, const META& a, const double* partials, int
   });
 }
 
+namespace {
+// f(first tile, workgroups) for one wave per tile in workgroups of one wave, at most kListMaxGrid of them per launch
+template <class F>
+hipError_t wave_per_tile(uint32_t n_tiles, F f) {
+  for (uint32_t first = 0; first < n_tiles; first += kListMaxGrid) {
+    const uint32_t left = n_tiles - first;
+    const hipError_t e = f(first, int(left < kListMaxGrid ? left : kListMaxGrid));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+static_assert(kListScaleBlock == 64 && kListAdamBlock == 64, "wave_per_tile counts workgroups of one wave");
+}  // namespace
+
 template <class META>
-hipError_t launch_list_scale(const META& a, const float* coef, int grid, hipStream_t stream) {
-  return launch_kernel(list_scale_kernel<META, kListScaleBlock>, grid, kListScaleBlock, stream, a, coef);
+hipError_t launch_list_scale(const META& a, const float* coef, hipStream_t stream) {
+  return wave_per_tile(a.n_tiles, [&](uint32_t first, int grid) {
+    return launch_kernel(list_scale_kernel<META, kListScaleBlock>, grid, kListScaleBlock, stream, a, first, coef);
+  });
 }
 
 namespace {
+template <class G, class O, class META>
+hipError_t adamw_go(const META& a, const AdamScalars& s, const float* grad_scale, hipStream_t stream) {
+  return wave_per_tile(a.n_tiles, [&](uint32_t first, int grid) {
+    return launch_kernel(list_adamw_kernel<G, O, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, first, s,
+                         grad_scale);
+  });
+}
 template <class G, class META>
-hipError_t adamw_by_out(int out_dt, const META& a, const AdamScalars& s, const float* grad_scale, int grid,
-                        hipStream_t stream) {
+hipError_t adamw_by_out(int out_dt, const META& a, const AdamScalars& s, const float* grad_scale, hipStream_t stream) {
   switch (out_dt) {
-    case DT_F32:
-      return launch_kernel(list_adamw_kernel<G, F32, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
-    case DT_BF16:
-      return launch_kernel(list_adamw_kernel<G, BF16, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
-    case DT_F16:
-      return launch_kernel(list_adamw_kernel<G, F16, META, kListAdamBlock>, grid, kListAdamBlock, stream, a, s, grad_scale);
+    case DT_F32: return adamw_go<G, F32>(a, s, grad_scale, stream);
+    case DT_BF16: return adamw_go<G, BF16>(a, s, grad_scale, stream);
+    case DT_F16: return adamw_go<G, F16>(a, s, grad_scale, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -90,11 +109,11 @@ hipError_t adamw_by_out(int out_dt, const META& a, const AdamScalars& s, const f
 
 template <class META>
 hipError_t launch_list_adamw(int grad_dt, int out_dt, const META& a, const AdamScalars& s, const float* grad_scale,
-                             int grid, hipStream_t stream) {
+                             hipStream_t stream) {
   switch (grad_dt) {
-    case DT_F32: return adamw_by_out<F32>(out_dt, a, s, grad_scale, grid, stream);
-    case DT_BF16: return adamw_by_out<BF16>(out_dt, a, s, grad_scale, grid, stream);
-    case DT_F16: return adamw_by_out<F16>(out_dt, a, s, grad_scale, grid, stream);
+    case DT_F32: return adamw_by_out<F32>(out_dt, a, s, grad_scale, stream);
+    case DT_BF16: return adamw_by_out<BF16>(out_dt, a, s, grad_scale, stream);
+    case DT_F16: return adamw_by_out<F16>(out_dt, a, s, grad_scale, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -102,13 +121,13 @@ hipError_t launch_list_adamw(int grad_dt, int out_dt, const META& a, const AdamS
 #define YAFSDP_LIST_INSTANCES(META)                                                                               \
   template hipError_t launch_list_norm<META>(int, const META&, double*, int, hipStream_t);                        \
   template hipError_t launch_list_clip<META>(int, const META&, const double*, int, float, float*, int, hipStream_t); \
-  template hipError_t launch_list_scale<META>(const META&, const float*, int, hipStream_t);
+  template hipError_t launch_list_scale<META>(const META&, const float*, hipStream_t);
 YAFSDP_LIST_INSTANCES(ListArgs)
 YAFSDP_LIST_INSTANCES(ListRef)
 #undef YAFSDP_LIST_INSTANCES
-template hipError_t launch_list_adamw<ListAdamArgs>(int, int, const ListAdamArgs&, const AdamScalars&, const float*, int,
+template hipError_t launch_list_adamw<ListAdamArgs>(int, int, const ListAdamArgs&, const AdamScalars&, const float*,
                                                     hipStream_t);
-template hipError_t launch_list_adamw<ListAdamRef>(int, int, const ListAdamRef&, const AdamScalars&, const float*, int,
+template hipError_t launch_list_adamw<ListAdamRef>(int, int, const ListAdamRef&, const AdamScalars&, const float*,
                                                    hipStream_t);
 
 }  // namespace yafsdp

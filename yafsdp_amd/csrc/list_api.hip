@@ -86,9 +86,9 @@ int check_disjoint(const std::vector<Range>& ranges) {
 }
 
 // workgroups of `block` lanes, one wave per tile, at most `cap`
-int grid_of(uint32_t n_tiles, int block, int64_t cap) {
+int grid_of(uint32_t n_tiles, int block, int cap) {
   const int per = block / 64;
-  return int(std::min((int64_t(n_tiles) + per - 1) / per, cap));
+  return int(std::min((int64_t(n_tiles) + per - 1) / per, int64_t(cap)));
 }
 
 constexpr size_t kPartialBytes = size_t(kListNormGrid) * sizeof(double);
@@ -99,12 +99,12 @@ size_t staged_bytes(size_t words) {
   return (words + kListStageWords - 1) / kListStageWords * kListStageWords * sizeof(uint32_t);
 }
 
-// The process's staging slots (never freed: kernels may read them until the end), or nullptr without pinned memory.
-// Call with the mutex of slots() held.
+// The process's staging slots (never freed: kernels may read them until the end).
 StageSlots& slots() {
   static StageSlots* s = new StageSlots;
   return *s;
 }
+// False without pinned memory; allocated at the first call.  Call with the slots' mutex held.
 bool have_slots(StageSlots& s) {
   static bool tried = false;
   if (!tried) {
@@ -164,7 +164,7 @@ int stage(const std::vector<uint32_t>& words, void* dst, hipStream_t stream) {
 }
 static_assert(StageSlots::kPieceBytes == size_t(kListFetchBlock) * 16, "a workgroup reads a piece");
 
-// Tile bookkeeping of range k: its tiles end at tile_end, its last one holds `tail`.
+// Tiles so far; false when a launch cannot count them.
 struct Tiles {
   uint64_t count = 0;
   bool add(uint64_t n) { return (count += n) <= uint64_t(INT32_MAX); }
@@ -230,7 +230,7 @@ int norm_or_clip_launches(const META& a, int norm, float max_norm, double* parti
                                 grid_of(a.n_tiles, kListClipBlock, kListClipGrid), stream));
   e = launch_list_finish(norm, partials, count, max_norm, norm_and_coef, stream);
   if (e != hipSuccess || !clip) return int(e);
-  return int(launch_list_scale(a, norm_and_coef + 1, grid_of(a.n_tiles, kListScaleBlock, INT32_MAX), stream));
+  return int(launch_list_scale(a, norm_and_coef + 1, stream));
 }
 
 int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
@@ -245,7 +245,7 @@ int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double m
   if (rc != YAFSDP_OK) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
     if constexpr (std::is_same<std::decay_t<decltype(a)>, ListArgs>::value)
-      if (a.n_tiles <= uint32_t(kListSmallTiles))
+      if (a.n_tiles <= uint32_t(clip ? kListSmallClipTiles : kListSmallNormTiles))
         return int(launch_list_small(norm, clip, a, static_cast<float>(max_norm), norm_and_coef, stream));
     return norm_or_clip_launches(a, norm, static_cast<float>(max_norm), static_cast<double*>(workspace), norm_and_coef,
                                  clip, stream);
@@ -291,7 +291,7 @@ int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* 
   if (rc == YAFSDP_OK) rc = check_disjoint(ranges);
   if (rc != YAFSDP_OK || ranges.empty()) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
-    return int(launch_list_scale(a, coef, grid_of(a.n_tiles, kListScaleBlock, INT32_MAX), stream));
+    return int(launch_list_scale(a, coef, stream));
   });
 } catch (...) {
   return YAFSDP_ERR_OUT_OF_MEMORY;
@@ -367,7 +367,6 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
     tail[i] = uint32_t(end - (t - 1) * kListAdamTile);
   }
   const uint32_t n_tiles = uint32_t(tiles.count);
-  const int grid = grid_of(n_tiles, kListAdamBlock, INT32_MAX);
   const auto record = [&](size_t i) {
     return ListAdamRange{ranges[i].p, ranges[i].g, ranges[i].m, ranges[i].v, ranges[i].out};
   };
@@ -380,7 +379,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
       a.tile_end[i] = tile_end[i];
       a.tail[i] = tail[i];
     }
-    return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, grid, stream));
+    return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, stream));
   }
   std::vector<uint32_t> words((kAdamRecordWords + 2) * k);
   for (size_t i = 0; i < k; i++) {
@@ -394,7 +393,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
   const uint32_t* base = static_cast<const uint32_t*>(workspace);
   const ListAdamRef a{int32_t(k), n_tiles, base + kAdamRecordWords * k, base + (kAdamRecordWords + 1) * k,
                       static_cast<const ListAdamRange*>(workspace)};
-  return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, grid, stream));
+  return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, stream));
 } catch (...) {
   return YAFSDP_ERR_OUT_OF_MEMORY;
 }

@@ -68,16 +68,33 @@ constexpr int kListFetchBlock = 1024;
 
 enum : int { LIST_NORM_1 = 1, LIST_NORM_2 = 2, LIST_NORM_INF = 3 };
 
+// ---- launch shapes, measured on MI355X (random data; times of whole calls) ------------------------------
+// Norm: a grid that loops, one partial sum per workgroup (kListNormGrid doubles of the caller's workspace).  Fewer waves
+// stream long ranges faster (436 MB in 9 ranges: 65.6 us with 512 workgroups, 68.4 with 1024), but where ranges are
+// short, so that a wave needs a new one for almost every tile, twice the waves hide the lookups (1427 ragged tensors,
+// 346 MB: 87 us and 68; 64 ranges of 8 MB: 84.7 and 82.4).  Long: at least kListNormLongRange tiles a range on average,
+// two strides of the smaller grid (16 ranges of 16 MB: 41.5 and 43.0).
 constexpr int kListNormBlock = 256;
-constexpr int kListNormGrid = 1024;  // = the most partial sums of one call (doubles in the caller's workspace)
+constexpr int kListNormGrid = 1024;
 constexpr int kListNormLongGrid = 512;
-constexpr int kListNormLongRange = 1024;
+constexpr int kListNormLongRange = 4096;
+// One workgroup for the whole call while that is faster than one launch more: norm of 128 tiles 11.8 us against 13.4, of
+// 256 tiles 18.6 against 14.0; clipping 64 tiles 11.4 against 13.6, 128 tiles 16.4 against 14.3.
 constexpr int kListSmallBlock = 1024;
-constexpr int kListSmallTiles = 128;
+constexpr int kListSmallNormTiles = 128;
+constexpr int kListSmallClipTiles = 96;
+// Scaling: one tile per wave and one wave per workgroup (1.74 GB: 570 us; two and four waves per workgroup 605 and 595,
+// grids that loop 670).  Up to kListClipTiles tiles a looping grid that also joins the partial sums saves the
+// finishing launch: 32 MB 22.5 -> 19.8 us, 134 MB 67.2 -> 67.0, beyond that it loses (268 MB 126 -> 128, 536 MB 246 -> 255).
 constexpr int kListScaleBlock = 64;
 constexpr int kListClipBlock = 256;
 constexpr int kListClipGrid = 1024;
 constexpr int kListClipTiles = 32768;
+// AdamW: one tile of 256 elements per wave, one wave per workgroup (a layer of 218 M elements, 6.1 GB: 1011 us; tiles
+// of 512 and 1024 elements 1038 and 1050; two and four waves per workgroup with tiles of 512 1051 and 1075).
 constexpr int kListAdamBlock = 64;
+// A grid has fewer than 2^32 lanes: a wave per tile takes several launches beyond this many (17 GB; 1.07 G elements of
+// AdamW).  (Waves that loop instead cost 0.4-1.5 % at every size.)
+constexpr uint32_t kListMaxGrid = 1u << 22;
 
 }  // namespace yafsdp

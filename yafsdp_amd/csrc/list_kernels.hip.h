@@ -1,8 +1,14 @@
 // Optimizer-side passes over a list of separate tensors: norm (1, 2, inf), scaling by a device-resident coefficient,
 // AdamW.  Nothing here is a contraction: all of it is bound by memory.
 //
-// Work is cut into wave-sized tiles (4 KiB for the norm and the scaling, 512 elements for AdamW); a wave finds the
-// range that holds its tile in the kernel arguments, which it reads through the constant address space (scalar loads).
+// Work is cut into wave-sized tiles (4 KiB for the norm and the scaling, 256 elements for AdamW); a wave looks the range
+// that holds its tile up by a binary search with scalar loads.  (Searching with one vector load and a ballot per 64
+// ranges measured slower: from the kernel arguments 97 us against 87 on 1427 tensors, because those are far away, and
+// from the workspace 74 against 69, because a vector load queues behind the data's.)
+//
+// Reached on MI355X (kernel alone): norm of 436 MB of bf16 6.7 TB/s and of 1.74 GB 6.9 TB/s (a read-only pass 7.2);
+// scaling 1.74 GB 6.3 TB/s (a copy 6.36); AdamW of 218 M elements 6.05 TB/s, with 573 ragged tensors 6.1 (a mover of its
+// streams without arithmetic 6.1-6.2).  What is left is the 4-5 us per launch that run below full rate.
 #pragma once
 #include "adam_elem.hip.h"
 #include "elem.hip.h"
@@ -361,13 +367,13 @@ __device__ __forceinline__ void scale_tile(const ListTile& x, const TileData& d,
   else scale_tile_of<F16>(x, d, c);
 }
 
-// one tile per wave
+// one tile per wave, from tile `first` on
 template <class META, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) list_scale_kernel(META meta, const float* coef) {
+__global__ void __launch_bounds__(BLOCK) list_scale_kernel(META meta, uint32_t first, const float* coef) {
   const float c = *as_const(coef);
   if (c == 1.0f) return;
   const ListView a = list_view(meta);
-  const uint32_t t = global_wave<BLOCK>();
+  const uint32_t t = first + global_wave<BLOCK>();
   if (t >= a.n_tiles) return;
   const ListTile x = TileCursor(a).tile(t);
   scale_tile(x, load_tile(x), c);
@@ -397,16 +403,16 @@ list_clip_kernel(META meta, const double* partials, int count, float max_norm, f
   stream_list<BLOCK>(a, [&](const ListTile& x, const TileData& d) { scale_tile(x, d, c); });
 }
 
-// A short list (at most kListSmallTiles tiles) in one launch of one workgroup: norm, coefficient and (CLIP) the scaling.
+// A short list (at most kListSmallNormTiles tiles) in one launch of one workgroup: norm, coefficient and (CLIP) the scaling.
 // The ranges' lanes first write every tile's place to LDS.  A wave scales the tiles it has read itself, so nothing but
 // the joined total passes between waves; the first kHeld tiles of a wave are loaded at once and stay in its registers.
 template <int NORM, bool CLIP, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) list_small_kernel(ListArgs, float max_norm, float* norm_and_coef) {
-  static_assert(BLOCK >= kListMax, "a lane per range");
+  static_assert(BLOCK >= kListMax && kListSmallClipTiles <= kListSmallNormTiles, "a lane per range, room for every tile");
   constexpr int kHeld = 4, kWaves = BLOCK / 64;
   __shared__ double lds[kWaves];
   __shared__ float shared_coef;
-  __shared__ ListTile tiles[kListSmallTiles];
+  __shared__ ListTile tiles[kListSmallNormTiles];
   const YAFSDP_CONST_AS ListArgs* a = first_argument<ListArgs>();
   const uint32_t n_tiles = a->n_tiles;
   const int i = threadIdx.x;
@@ -447,9 +453,11 @@ __global__ void __launch_bounds__(BLOCK) list_small_kernel(ListArgs, float max_n
 }
 
 // ------------------------------------------------------------------ AdamW ----
-// adam_elem on each element: same operations, same roundings, same bits as adamw_kernel.  A
-// 16-bit gradient enters as the binary32 number it stands for; its product with grad_scale is rounded to binary32 (a
-// grad.mul_ beforehand would round it to 16 bits).  O is F32 for "no 16-bit copy".
+// adam_elem on each element: same operations, same roundings, same bits as adamw_kernel.  A 16-bit gradient enters as
+// the binary32 number it stands for; its product with grad_scale is rounded to binary32 (a grad.mul_ beforehand would
+// round it to 16 bits).  O is F32 for "no 16-bit copy".  Tiles are counted from a 256-byte boundary of the parameters:
+// with tiles from the first element of each tensor, two waves share a line at every tile's ends in all four or five
+// arrays, and 573 ragged tensors took 280 us instead of 222.
 template <class G>
 __device__ __forceinline__ float adam_grad(float g) {
   if constexpr (G::kId == DT_F16) return opaque(g);
@@ -468,13 +476,15 @@ __device__ __forceinline__ void store_nt(YAFSDP_GLOBAL_AS typename T::storage* p
   __builtin_nontemporal_store(q.v, (YAFSDP_GLOBAL_AS typename T::quad_unaligned*)p);
 }
 
+// one tile per wave, from tile `first_tile` on
 template <class G, class O, class META, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) list_adamw_kernel(META meta, AdamScalars s, const float* grad_scale) {
+__global__ void __launch_bounds__(BLOCK)
+list_adamw_kernel(META meta, uint32_t first_tile, AdamScalars s, const float* grad_scale) {
   constexpr bool kOut = !same_t<O, F32>::value;
   static_assert(kListAdamTile == 256, "a wave holds a tile as one quad per lane");
   typedef typename G::storage g_t;
   const ListAdamView a = list_view(meta);
-  const uint32_t t = global_wave<BLOCK>();
+  const uint32_t t = first_tile + global_wave<BLOCK>();
   if (t >= a.n_tiles) return;
   const bool scaled = grad_scale != nullptr;
   float gs = 1.0f;

@@ -280,6 +280,17 @@ def zero_grad(modules: nn.Module | Iterable[nn.Module]) -> None:
         _native.flat_fill(group._padded_sharded_param_grad[key], 0.0)
 
 
+def _check_hyperparameters(lr, betas: tuple[float, float], eps: float, weight_decay: float) -> None:
+    if not 0.0 <= float(lr):
+        raise ValueError(f"Invalid learning rate: {lr}")
+    if not 0.0 <= eps:
+        raise ValueError(f"Invalid epsilon value: {eps}")
+    if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+        raise ValueError(f"Invalid beta parameters: {betas}")
+    if not 0.0 <= weight_decay:
+        raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+
+
 def _resolve(t: torch.Tensor) -> torch.Tensor:
     """The plain tensor behind a sharded parameter or gradient: this rank's fragment."""
     return plain_tensor(local_tensor(t)) if isinstance(t, torch.Tensor) else t
@@ -342,6 +353,7 @@ def list_adamw_step(
     first, in binary32, without writing it back; ``zero_grad=True`` zero-fills the gradients in the same pass.  Per
     element the arithmetic is that of ``FlatAdamW``, bit for bit.  All tensors are contiguous, live on one GPU, and what
     is written shares no memory with anything else in the lists."""
+    _check_hyperparameters(lr, betas, eps, weight_decay)
     if step < 1:
         raise ValueError(f"Invalid step: {step}")
     lst = _native.AdamwList(params, grads, exp_avgs, exp_avg_sqs, outs16, _resolve)
@@ -419,14 +431,7 @@ class FlatAdamW(torch.optim.Optimizer):
         decoupled_weight_decay: bool = True,
         fuse_copy_in: bool = True,
     ):
-        if not 0.0 <= float(lr):
-            raise ValueError(f"Invalid learning rate: {lr}")
-        if not 0.0 <= eps:
-            raise ValueError(f"Invalid epsilon value: {eps}")
-        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
-            raise ValueError(f"Invalid beta parameters: {betas}")
-        if not 0.0 <= weight_decay:
-            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        _check_hyperparameters(lr, betas, eps, weight_decay)
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                         decoupled_weight_decay=decoupled_weight_decay)
         super().__init__(params, defaults)
