@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 from typing import Sequence
@@ -246,6 +247,13 @@ def _stream(t: torch.Tensor) -> int:
         index = t.device.index
         return _raw_current_stream(torch.cuda.current_device() if index is None else index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _device_stream(device: torch.device) -> int:
+    """The same for a device with an index."""
+    if _raw_current_stream is not None:
+        return _raw_current_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _on(device: torch.device):
@@ -927,6 +935,12 @@ _ADAMW_ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("exp_avg", 
                          ("out16", np.uint64), ("numel", np.int64)])
 
 
+# looked up once per count / index: 0.7 us each through ctypes and torch
+_list_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.yafsdp_list_workspace_bytes)
+_list_adamw_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.yafsdp_list_adamw_workspace_bytes)
+_cuda_device = functools.lru_cache(maxsize=None)(functools.partial(torch.device, "cuda"))
+
+
 def _is_dense(t: torch.Tensor) -> bool:
     """Whether the elements fill one range of memory, each once, in whatever order of the dimensions."""
     if t.is_contiguous():
@@ -973,7 +987,7 @@ class TensorList:
         if got is not None:
             self.tensors = tensors
             self.entries, self.count, index = got
-            self.device = torch.device("cuda", index)
+            self.device = _cuda_device(index)
             return
         # not accepted as it stands: resolve wrappers, find out what is wrong and raise
         if resolve is not None:
@@ -1019,14 +1033,14 @@ def _list_norm(fn, name: str, lst: TensorList, norm_type, max_norm: float) -> to
     with _on(lst.device):
         _check(
             fn(lst.entries, lst.count, code, float(max_norm), workspace.data_ptr(), nbytes, norm_and_coef.data_ptr(),
-               _stream(norm_and_coef)),
+               _device_stream(lst.device)),
             name,
         )
     return norm_and_coef
 
 
 def _list_workspace(lst: TensorList) -> "tuple[torch.Tensor, int]":
-    nbytes = lib.yafsdp_list_workspace_bytes(lst.count)
+    nbytes = _list_workspace_bytes(lst.count)
     return torch.empty(nbytes, dtype=torch.uint8, device=lst.device), nbytes
 
 
@@ -1068,7 +1082,7 @@ class AdamwList:
         if got is not None:
             self.lists = lists
             self.entries, self.count, index, self.grad_code, self.out_code = got
-            self.device = torch.device("cuda", index)
+            self.device = _cuda_device(index)
             return
         if resolve is not None:
             lists = [None if ts is None else [None if t is None else resolve(t) for t in ts] for ts in lists]
@@ -1132,14 +1146,13 @@ def list_adamw(
             raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
         gs_ptr = grad_scale.data_ptr()
     flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
-    need = lib.yafsdp_list_adamw_workspace_bytes(lst.count)
+    need = _list_adamw_workspace_bytes(lst.count)
     workspace = torch.empty(need, dtype=torch.uint8, device=lst.device) if need else None
     with _on(lst.device):
-        stream = _raw_current_stream(lst.device.index) if _raw_current_stream is not None else (
-            torch.cuda.current_stream(lst.device).cuda_stream)
         code = lib.yafsdp_list_adamw(
             lst.entries, lst.count, lst.grad_code, lst.out_code, float(lr), float(beta1), float(beta2), float(eps),
-            float(weight_decay), int(step), gs_ptr, flags, workspace.data_ptr() if need else None, need, stream,
+            float(weight_decay), int(step), gs_ptr, flags, workspace.data_ptr() if need else None, need,
+            _device_stream(lst.device),
         )
     if code == ERR_OVERLAP and allow_overlap:
         return False
