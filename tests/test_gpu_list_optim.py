@@ -223,6 +223,38 @@ def test_clip_of_many_tensors_of_every_dtype():
             assert_bits_equal(a, b, f"tensor {i}")
 
 
+@pytest.mark.parametrize("order", ["ascending", "descending"])
+def test_clip_of_neighbours_of_other_dtypes(order):
+    """Tensors of all dtypes back to back in one allocation: several of them inside one 16-byte vector, tiles of
+    different waves in one cache line."""
+    from yafsdp_amd.optim import list_clip_grad_norm_
+
+    gen = torch.Generator().manual_seed(14)
+    sizes = [1, 2, 3, 1, 5, 1, 1, 2, 9, 700, 1, 4096, 33, 2, 1, 6000] * 12
+    raw = torch.zeros(200_000 * 4, dtype=torch.uint8)
+    cpu, spans, at = [], [], 4
+    for i, n in enumerate(sizes):
+        dtype = DTYPES[i % 3]
+        size = 4 if dtype == F32 else 2
+        at = -(-at // size) * size
+        t = raw[at:at + n * size].view(dtype)
+        t.copy_(torch.randn(n, generator=gen))
+        cpu.append(t)
+        spans.append((at, n, size, dtype))
+        at += n * size
+    dev_raw = raw.to(DEV)
+    dev = [dev_raw[a:a + n * size].view(dtype) for a, n, size, dtype in spans]
+    if order == "descending":
+        dev.reverse()
+    norm = list_clip_grad_norm_(dev, 2.0)
+    _assert_norm(norm, cpu, 2.0)
+    for t in cpu:
+        part = t.clone()
+        cref.flat_scale(part, _coef32(norm.item(), 2.0))
+        t.copy_(part)
+    assert torch.equal(dev_raw.cpu(), raw)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_clip_of_special_values(dtype):
     """Subnormals, signed zeros, ties: x * c in binary32, rounded once."""
@@ -530,6 +562,41 @@ def test_more_long_lists_in_flight_than_staging_slots():
         _oracle_step(cpu, starts, numels, None, False, step=2, grad_scale=float(coef), **CHP)
         for k in "pmv":
             assert_bits_equal(dev[k], cpu[k], k)
+
+
+def test_list_longer_than_a_staging_slot():
+    """11,000 tensors of AdamW (528 KB of list) travel in kernel arguments; the norm of the same gradients (176 KB) fits."""
+    from yafsdp_amd.optim import list_adamw_step, list_clip_coef
+
+    numels = [1 + i % 3 for i in range(11_000)]
+    cpu, starts = _adam_case(numels, BF16, None, 1, 0, 15)
+    dev = {k: b.to(DEV) for k, b in cpu.items()}
+    lists = {k: _views(b, starts, numels) for k, b in dev.items()}
+    norm, coef = list_clip_coef(lists["g"], 0.1)
+    list_adamw_step(lists["p"], lists["g"], lists["m"], lists["v"], step=2, grad_scale=coef, **HP)
+    _assert_norm(norm, _views(cpu["g"], starts, numels), 2.0)
+    live = torch.zeros(cpu["p"].numel(), dtype=torch.bool)
+    for s, n in zip(starts, numels):
+        live[s:s + n] = True
+    part = {k: cpu[k][live].float() for k in "pgmv"}  # elementwise: all tensors as one
+    cref.adamw_step(part["p"], part["g"], part["m"], part["v"], None, step=2, grad_scale=float(coef), **CHP)
+    for k in "pmv":
+        cpu[k][live] = part[k]
+        assert_bits_equal(dev[k], cpu[k], k)
+
+
+def test_kernel_timing_hook_covers_list_launches():
+    from yafsdp_amd import _native
+    from yafsdp_amd.optim import list_grad_norm
+
+    ts = [torch.randn(n, device=DEV) for n in (1_000_000, 77)]
+    want = list_grad_norm(ts)
+    start, stop = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    _native.time_next_launch(start, stop)
+    got = list_grad_norm(ts)
+    torch.cuda.synchronize()
+    assert 0.0 < start.elapsed_time(stop) < 1000.0
+    assert_bits_equal(got, want, "timed launch")
 
 
 def test_captured_step_replays_with_new_gradients():

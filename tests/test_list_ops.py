@@ -213,6 +213,13 @@ def test_adamw_entries_of_cpu_tensors():
     assert tl.adamw_entries(ps, gs, ms, vs[:2], None, False) is None
 
 
+def test_whole_calls_hand_back_what_they_do_not_take():
+    """Nothing is called for a list that is not on the GPU asked for (the addresses here are not code)."""
+    a = [torch.zeros(3)]
+    assert tl.list_norm(8, 8, a, 0, 0, 2, 1.0) is None and tl.list_norm(8, 8, [], 0, 0, 2, 1.0) is None
+    assert tl.list_adamw(8, 8, a, a, a, a, None, 0, 0, 1e-3, 0.9, 0.9, 1e-8, 0.0, 1, 0, 0) is None
+
+
 def test_bump_versions_matches_torch():
     base = torch.zeros(8)
     a, b = base[:4], torch.zeros(3)

@@ -25,10 +25,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("YAFSDP_HIP_LIBRARY") or os.path.join(_HERE, "libyafsdp_hip.so")
 
 # optional host-side helper (csrc/tensorlist.cpp): validates a tensor list and writes its pointer array in one
-# C++ pass; without it the same checks run in Python.  It launches nothing and touches no tensor data.
+# C++ pass; without it the same checks run in Python.  It touches no tensor data.
 try:
     from . import _tensorlist
-except ImportError:  # not built: the Python checks below do the same work, slower for large tables
+except ImportError:  # not built: the Python code below does the same work, slower
     _tensorlist = None
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -1006,12 +1006,9 @@ class TensorList:
         self.tensors = tensors
         self.entries, self.count, self.device = np.array(rows, dtype=_LIST_ENTRY).tobytes(), len(rows), device
 
-    def bump_versions(self) -> None:
-        """What an in-place torch op does to its tensors' version counters."""
-        _bump_versions(self.tensors)
-
 
 def _bump_versions(tensors, where=None) -> None:
+    """What an in-place torch op does to its tensors' version counters (where ``where`` is not None)."""
     if _tensorlist is not None:
         _tensorlist.bump_versions(tensors, where)
         return
@@ -1026,8 +1023,33 @@ def norm_code(norm_type) -> int:
         raise NotImplementedError(f"only the 1-, 2- and infinity-norm are implemented, got {norm_type}") from None
 
 
-def _list_norm(fn, name: str, lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
-    code = norm_code(norm_type)
+def _list_workspace(lst: TensorList) -> "tuple[torch.Tensor, int]":
+    nbytes = _list_workspace_bytes(lst.count)
+    return torch.empty(nbytes, dtype=torch.uint8, device=lst.device), nbytes
+
+
+def _address(fn) -> int:
+    return ctypes.cast(fn, ctypes.c_void_p).value
+
+
+_LIST_NORM = (lib.yafsdp_list_norm, _address(lib.yafsdp_list_norm), "yafsdp_list_norm")
+_LIST_CLIP = (lib.yafsdp_list_clip, _address(lib.yafsdp_list_clip), "yafsdp_list_clip")
+_LIST_WS, _ADAMW_WS = _address(lib.yafsdp_list_workspace_bytes), _address(lib.yafsdp_list_adamw_workspace_bytes)
+_LIST_ADAMW = _address(lib.yafsdp_list_adamw)
+
+
+def _list_norm(entry, tensors, norm_type, max_norm: float, what: str, resolve) -> "tuple[torch.Tensor, Sequence]":
+    fn, address, name = entry
+    code, tensors = norm_code(norm_type), _as_list(tensors, what)
+    if _tensorlist is not None and _raw_current_stream is not None:  # plain tensors on the current device
+        index = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+        if index >= 0:
+            got = _tensorlist.list_norm(address, _LIST_WS, tensors, index, _raw_current_stream(index), code,
+                                        float(max_norm))
+            if got is not None:
+                _check(got[0], name)
+                return got[1], tensors
+    lst = TensorList(tensors, what, resolve)
     norm_and_coef = torch.empty(2, dtype=torch.float32, device=lst.device)
     workspace, nbytes = _list_workspace(lst)
     with _on(lst.device):
@@ -1036,22 +1058,20 @@ def _list_norm(fn, name: str, lst: TensorList, norm_type, max_norm: float) -> to
                _device_stream(lst.device)),
             name,
         )
-    return norm_and_coef
+    return norm_and_coef, lst.tensors
 
 
-def _list_workspace(lst: TensorList) -> "tuple[torch.Tensor, int]":
-    nbytes = _list_workspace_bytes(lst.count)
-    return torch.empty(nbytes, dtype=torch.uint8, device=lst.device), nbytes
+def list_norm(tensors, norm_type, max_norm: float, what: str = "tensors", resolve=None) -> torch.Tensor:
+    """``[norm, clip coefficient]`` (float32) over every element of a list (see ``TensorList``); ``norm_type`` 1, 2 or
+    infinity."""
+    return _list_norm(_LIST_NORM, tensors, norm_type, max_norm, what, resolve)[0]
 
 
-def list_norm(lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
-    """``[norm, clip coefficient]`` (float32) over every element of the list; ``norm_type`` 1, 2 or infinity."""
-    return _list_norm(lib.yafsdp_list_norm, "yafsdp_list_norm", lst, norm_type, max_norm)
-
-
-def list_clip(lst: TensorList, norm_type, max_norm: float) -> torch.Tensor:
+def list_clip(tensors, norm_type, max_norm: float, what: str = "tensors", resolve=None) -> torch.Tensor:
     """``list_norm``, then every element times the coefficient, in place."""
-    return _list_norm(lib.yafsdp_list_clip, "yafsdp_list_clip", lst, norm_type, max_norm)
+    norm_and_coef, tensors = _list_norm(_LIST_CLIP, tensors, norm_type, max_norm, what, resolve)
+    _bump_versions(tensors)
+    return norm_and_coef
 
 
 def list_scale(lst: TensorList, coef: torch.Tensor) -> None:
@@ -1124,39 +1144,52 @@ class AdamwList:
         self.entries, self.count, self.device = np.array(rows, dtype=_ADAMW_ENTRY).tobytes(), len(rows), device
         self.grad_code, self.out_code = DTYPE_CODE[grad_dtype], 0 if out_dtype is None else DTYPE_CODE[out_dtype]
 
-    def bump_versions(self, zero_grad: bool) -> None:
-        """Of everything the step writes: the positions with a gradient of every list but the gradients (of those too
-        where the step zero-fills them)."""
-        params, grads, exp_avgs, exp_avg_sqs, outs16 = self.lists
-        for ts in (params, grads if zero_grad else None, exp_avgs, exp_avg_sqs, outs16):
-            if ts is not None:
-                _bump_versions(ts, grads)
-
 
 def list_adamw(
-    lst: AdamwList, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: int,
-    decoupled: bool = True, grad_scale: torch.Tensor | None = None, zero_grad: bool = False, allow_overlap: bool = False,
+    params, grads, exp_avgs, exp_avg_sqs, outs16=None, resolve=None, *, lr: float, beta1: float, beta2: float, eps: float,
+    weight_decay: float, step: int, decoupled: bool = True, grad_scale: torch.Tensor | None = None, zero_grad: bool = False,
+    bump_versions: bool = True, allow_overlap: bool = False,
 ) -> bool:
-    """One Adam(W) step on every position of the lists, with the bits of ``adamw_step``.  Tensors that the step writes
-    must not share memory: refused, or with ``allow_overlap`` reported by returning False with nothing launched."""
-    gs_ptr = None
+    """One Adam(W) step on every position of the lists (see ``AdamwList``), with the bits of ``adamw_step``.  Tensors that
+    the step writes must not share memory: refused, or with ``allow_overlap`` reported by returning False with nothing
+    launched."""
+    gs_ptr = 0
     if grad_scale is not None:
         _flat_arg(grad_scale, "grad_scale")
-        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != lst.device:
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
         gs_ptr = grad_scale.data_ptr()
     flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
-    need = _list_adamw_workspace_bytes(lst.count)
-    workspace = torch.empty(need, dtype=torch.uint8, device=lst.device) if need else None
-    with _on(lst.device):
-        code = lib.yafsdp_list_adamw(
-            lst.entries, lst.count, lst.grad_code, lst.out_code, float(lr), float(beta1), float(beta2), float(eps),
-            float(weight_decay), int(step), gs_ptr, flags, workspace.data_ptr() if need else None, need,
-            _device_stream(lst.device),
-        )
+    lists = [_as_list(ts, name) for ts, name in zip((params, grads, exp_avgs, exp_avg_sqs), AdamwList._NAMES)]
+    lists.append(None if outs16 is None else _as_list(outs16, "outs16"))
+    code = None
+    if _tensorlist is not None and _raw_current_stream is not None:  # plain tensors on the current device
+        index = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+        if index >= 0 and (grad_scale is None or grad_scale.device.index == index):
+            code = _tensorlist.list_adamw(
+                _LIST_ADAMW, _ADAMW_WS, *lists, index, _raw_current_stream(index), float(lr), float(beta1), float(beta2),
+                float(eps), float(weight_decay), int(step), gs_ptr, flags)
+    if code is None:
+        lst = AdamwList(*lists, resolve)
+        if grad_scale is not None and grad_scale.device != lst.device:
+            raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
+        need = _list_adamw_workspace_bytes(lst.count)
+        workspace = torch.empty(need, dtype=torch.uint8, device=lst.device) if need else None
+        with _on(lst.device):
+            code = lib.yafsdp_list_adamw(
+                lst.entries, lst.count, lst.grad_code, lst.out_code, float(lr), float(beta1), float(beta2), float(eps),
+                float(weight_decay), int(step), gs_ptr or None, flags, workspace.data_ptr() if need else None, need,
+                _device_stream(lst.device),
+            )
+        lists = lst.lists
     if code == ERR_OVERLAP and allow_overlap:
         return False
     _check(code, "yafsdp_list_adamw")
+    if bump_versions:
+        grads = lists[1]
+        for ts in (lists[0], grads if zero_grad else None, *lists[2:]):
+            if ts is not None:
+                _bump_versions(ts, grads)
     return True
 
 

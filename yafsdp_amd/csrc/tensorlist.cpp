@@ -5,15 +5,16 @@
 // The same checks written in Python cost about 0.6 us per tensor (five
 // interpreter-level passes); a parameter group with 1,400 tensors then spends
 // longer on the host than its kernel runs.  This pass takes about 10 ns per
-// tensor.  It moves no tensor data and launches nothing; the kernels and the
-// C ABI stay free of torch types.  Any list it does not accept is handed back to
-// the Python checks, which raise the descriptive error.
+// tensor.  It moves no tensor data; the kernels and the C ABI stay free of torch
+// types (the list calls reach the ABI through addresses that the binding passes).
+// Any list it does not accept is handed back to the Python checks, which raise
+// the descriptive error.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <cstdint>
-#include <string>
+#include <vector>
 
 #include "../../include/yafsdp_hip.h"
 
@@ -109,73 +110,94 @@ inline const at::Tensor* plain_tensor(PyObject* o, bool want_cuda, int64_t& devi
   return dev.index() == device_index ? &t : nullptr;
 }
 
-// (entries, count, device index) of a list of tensors, None entries left out; None if the list is not accepted as it
-// stands.  Elementwise and order-free passes: any dense layout will do, whatever its dimension order.
-py::object list_entries(py::handle tensors, bool want_cuda) {
-  PyObject* seq = tensors.ptr();
-  if (!PyList_Check(seq) && !PyTuple_Check(seq)) return py::none();
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
-  PyObject** items = PySequence_Fast_ITEMS(seq);
-  std::string buf(size_t(n) * sizeof(yafsdp_list_entry), '\0');
-  auto* out = reinterpret_cast<yafsdp_list_entry*>(&buf[0]);
-  int64_t device_index = -2, count = 0;
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    if (items[i] == Py_None) continue;
-    const at::Tensor* t = plain_tensor(items[i], want_cuda, device_index);
-    if (t == nullptr) return py::none();
-    const int code = dtype_code(t->scalar_type());
-    if (code < 0 || !t->is_non_overlapping_and_dense()) return py::none();
-    out[count++] = yafsdp_list_entry{t->numel() ? t->data_ptr() : nullptr, t->numel(), code, 0};
+struct ListEntries {
+  std::vector<yafsdp_list_entry> entries;  // None left out
+  int64_t device_index = -2;
+
+  // False if the list is not accepted as it stands.  Elementwise and order-free passes: any dense layout will do,
+  // whatever its dimension order.
+  bool collect(py::handle tensors, bool want_cuda) {
+    PyObject* seq = tensors.ptr();
+    if (!PyList_Check(seq) && !PyTuple_Check(seq)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    PyObject** items = PySequence_Fast_ITEMS(seq);
+    entries.reserve(size_t(n));
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      if (items[i] == Py_None) continue;
+      const at::Tensor* t = plain_tensor(items[i], want_cuda, device_index);
+      if (t == nullptr) return false;
+      const int code = dtype_code(t->scalar_type());
+      if (code < 0 || !t->is_non_overlapping_and_dense()) return false;
+      entries.push_back(yafsdp_list_entry{t->numel() ? t->data_ptr() : nullptr, t->numel(), code, 0});
+    }
+    return !entries.empty();
   }
-  if (count == 0) return py::none();
-  return py::make_tuple(py::bytes(buf.data(), size_t(count) * sizeof(yafsdp_list_entry)), count, device_index);
+};
+
+// (entries, count, device index) of a list of tensors; None if the list is not accepted as it stands.
+py::object list_entries(py::handle tensors, bool want_cuda) {
+  ListEntries l;
+  if (!l.collect(tensors, want_cuda)) return py::none();
+  return py::make_tuple(
+      py::bytes(reinterpret_cast<const char*>(l.entries.data()), l.entries.size() * sizeof(yafsdp_list_entry)),
+      l.entries.size(), l.device_index);
 }
 
-// (entries, count, device index, gradient dtype code, 16-bit copy's dtype code or 0) of five parallel lists; positions
-// without a gradient are left out.  `outs`: None for "no 16-bit copies".  None if not accepted as they stand.
+struct AdamwEntries {
+  std::vector<yafsdp_adamw_entry> entries;  // positions without a gradient and empty ones left out
+  int64_t device_index = -2;
+  int grad_code = -1, out_code = 0;
+
+  // Five parallel lists; `outs`: None for "no 16-bit copies".  False if not accepted as they stand.
+  bool collect(py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs, py::handle outs,
+               bool want_cuda) {
+    const bool has_out = !outs.is_none();
+    PyObject* seqs[5] = {params.ptr(), grads.ptr(), exp_avgs.ptr(), exp_avg_sqs.ptr(), outs.ptr()};
+    const int lists = has_out ? 5 : 4;
+    PyObject** items[5] = {};
+    Py_ssize_t n = -1;
+    for (int k = 0; k < lists; ++k) {
+      if (!PyList_Check(seqs[k]) && !PyTuple_Check(seqs[k])) return false;
+      if (n >= 0 && PySequence_Fast_GET_SIZE(seqs[k]) != n) return false;
+      n = PySequence_Fast_GET_SIZE(seqs[k]);
+      items[k] = PySequence_Fast_ITEMS(seqs[k]);
+    }
+    entries.reserve(size_t(n));
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      if (items[1][i] == Py_None) continue;
+      const at::Tensor* t[5] = {};
+      for (int k = 0; k < lists; ++k) {
+        t[k] = plain_tensor(items[k][i], want_cuda, device_index);
+        if (t[k] == nullptr || t[k]->numel() != t[0]->numel() || !t[k]->is_contiguous()) return false;
+      }
+      for (int k : {0, 2, 3})
+        if (t[k]->scalar_type() != at::kFloat) return false;
+      const int g = dtype_code(t[1]->scalar_type());
+      if (g < 0 || (grad_code >= 0 && g != grad_code)) return false;
+      grad_code = g;
+      if (has_out) {
+        const int o = dtype_code(t[4]->scalar_type());
+        if (o <= 0 || (out_code > 0 && o != out_code)) return false;
+        out_code = o;
+      }
+      const int64_t numel = t[0]->numel();
+      if (numel == 0) continue;
+      entries.push_back(yafsdp_adamw_entry{static_cast<float*>(t[0]->data_ptr()), t[1]->data_ptr(),
+                                           static_cast<float*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
+                                           has_out ? t[4]->data_ptr() : nullptr, numel});
+    }
+    return grad_code >= 0;
+  }
+};
+
+// (entries, count, device index, gradient dtype code, 16-bit copy's dtype code or 0); None if not accepted.
 py::object adamw_entries(py::handle params, py::handle grads, py::handle exp_avgs, py::handle exp_avg_sqs,
                          py::handle outs, bool want_cuda) {
-  const bool has_out = !outs.is_none();
-  PyObject* seqs[5] = {params.ptr(), grads.ptr(), exp_avgs.ptr(), exp_avg_sqs.ptr(), outs.ptr()};
-  const int lists = has_out ? 5 : 4;
-  PyObject** items[5] = {};
-  Py_ssize_t n = -1;
-  for (int k = 0; k < lists; ++k) {
-    if (!PyList_Check(seqs[k]) && !PyTuple_Check(seqs[k])) return py::none();
-    if (n >= 0 && PySequence_Fast_GET_SIZE(seqs[k]) != n) return py::none();
-    n = PySequence_Fast_GET_SIZE(seqs[k]);
-    items[k] = PySequence_Fast_ITEMS(seqs[k]);
-  }
-  std::string buf(size_t(n) * sizeof(yafsdp_adamw_entry), '\0');
-  auto* out = reinterpret_cast<yafsdp_adamw_entry*>(&buf[0]);
-  int64_t device_index = -2, count = 0;
-  int grad_code = -1, out_code = 0;
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    if (items[1][i] == Py_None) continue;
-    const at::Tensor* t[5] = {};
-    for (int k = 0; k < lists; ++k) {
-      t[k] = plain_tensor(items[k][i], want_cuda, device_index);
-      if (t[k] == nullptr || t[k]->numel() != t[0]->numel() || !t[k]->is_contiguous()) return py::none();
-    }
-    for (int k : {0, 2, 3})
-      if (t[k]->scalar_type() != at::kFloat) return py::none();
-    const int g = dtype_code(t[1]->scalar_type());
-    if (g < 0 || (grad_code >= 0 && g != grad_code)) return py::none();
-    grad_code = g;
-    if (has_out) {
-      const int o = dtype_code(t[4]->scalar_type());
-      if (o <= 0 || (out_code > 0 && o != out_code)) return py::none();
-      out_code = o;
-    }
-    const int64_t numel = t[0]->numel();
-    if (numel == 0) continue;
-    out[count++] = yafsdp_adamw_entry{static_cast<float*>(t[0]->data_ptr()), t[1]->data_ptr(),
-                                      static_cast<float*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
-                                      has_out ? t[4]->data_ptr() : nullptr, numel};
-  }
-  if (grad_code < 0) return py::none();
-  return py::make_tuple(py::bytes(buf.data(), size_t(count) * sizeof(yafsdp_adamw_entry)), count, device_index,
-                        grad_code, out_code);
+  AdamwEntries l;
+  if (!l.collect(params, grads, exp_avgs, exp_avg_sqs, outs, want_cuda)) return py::none();
+  return py::make_tuple(
+      py::bytes(reinterpret_cast<const char*>(l.entries.data()), l.entries.size() * sizeof(yafsdp_adamw_entry)),
+      l.entries.size(), l.device_index, l.grad_code, l.out_code);
 }
 
 // What an in-place torch op does to its tensors' version counters (the kernels write behind autograd's back).  With
@@ -196,6 +218,53 @@ void bump_versions(py::handle tensors, py::handle where) {
   }
 }
 
+// ---- whole calls, for lists on the current device ---------------------------------------------------------------
+// What the Python binding does through ctypes in 5-6 us (entries as bytes, two torch.empty, argument conversion) takes
+// about 2 us here.  `fn` / `ws_fn`: addresses of the ABI's entry point and of its workspace size.
+inline at::Tensor scratch(uint64_t ws_fn, int64_t count, int64_t device_index) {
+  const size_t bytes = reinterpret_cast<size_t (*)(int64_t)>(ws_fn)(count);
+  return at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c10::DeviceIndex(device_index)));
+}
+
+// yafsdp_list_norm / yafsdp_list_clip: (status, [norm, coefficient] tensor), or None if the list is not accepted.
+py::object list_norm(uint64_t fn, uint64_t ws_fn, py::handle tensors, int64_t device_index, uint64_t stream, int norm,
+                     double max_norm) {
+  ListEntries l;
+  if (!l.collect(tensors, true) || l.device_index != device_index) return py::none();
+  const int64_t count = int64_t(l.entries.size());
+  const at::Tensor ws = scratch(ws_fn, count, device_index);
+  at::Tensor out = at::empty({2}, ws.options().dtype(at::kFloat));
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = reinterpret_cast<decltype(&yafsdp_list_norm)>(fn)(l.entries.data(), count, norm, max_norm, ws.data_ptr(),
+                                                               size_t(ws.numel()), out.data_ptr<float>(),
+                                                               reinterpret_cast<void*>(stream));
+  }
+  return py::make_tuple(status, out);
+}
+
+// yafsdp_list_adamw: its status, or None if the lists are not accepted.
+py::object list_adamw(uint64_t fn, uint64_t ws_fn, py::handle params, py::handle grads, py::handle exp_avgs,
+                      py::handle exp_avg_sqs, py::handle outs, int64_t device_index, uint64_t stream, double lr,
+                      double beta1, double beta2, double eps, double weight_decay, int64_t step, uint64_t grad_scale,
+                      int flags) {
+  AdamwEntries l;
+  if (!l.collect(params, grads, exp_avgs, exp_avg_sqs, outs, true) || l.device_index != device_index) return py::none();
+  const int64_t count = int64_t(l.entries.size());
+  at::Tensor ws;
+  if (reinterpret_cast<size_t (*)(int64_t)>(ws_fn)(count) > 0) ws = scratch(ws_fn, count, device_index);
+  int status;
+  {
+    py::gil_scoped_release release;
+    status = reinterpret_cast<decltype(&yafsdp_list_adamw)>(fn)(
+        l.entries.data(), count, l.grad_code, l.out_code, lr, beta1, beta2, eps, weight_decay, step,
+        reinterpret_cast<const float*>(grad_scale), flags, ws.defined() ? ws.data_ptr() : nullptr,
+        ws.defined() ? size_t(ws.numel()) : 0, reinterpret_cast<void*>(stream));
+  }
+  return py::int_(status);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tensorlist, m) {
@@ -204,5 +273,7 @@ PYBIND11_MODULE(_tensorlist, m) {
   m.def("all_contiguous", &all_contiguous);
   m.def("list_entries", &list_entries, "yafsdp_list_entry array of a list of tensors");
   m.def("adamw_entries", &adamw_entries, "yafsdp_adamw_entry array of parallel lists of tensors");
+  m.def("list_norm", &list_norm);
+  m.def("list_adamw", &list_adamw);
   m.def("bump_versions", &bump_versions, py::arg("tensors"), py::arg("where") = py::none());
 }

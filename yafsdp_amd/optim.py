@@ -308,7 +308,7 @@ def list_clip_coef(
     is 1, 2 or infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64
     and are reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls;
     the call can be captured into a HIP graph, which then reads the same addresses at every replay."""
-    return _native.list_norm(_native.TensorList(grads, "grads", _resolve), norm_type, max_norm).unbind()
+    return _native.list_norm(grads, norm_type, max_norm, "grads", _resolve).unbind()
 
 
 def list_grad_norm(grads: Iterable[torch.Tensor | None], norm_type: float = 2.0) -> torch.Tensor:
@@ -322,10 +322,7 @@ def list_clip_grad_norm_(
     """``torch.nn.utils.clip_grad_norm_`` over a list of gradients (see ``list_clip_coef``): every element is multiplied
     by the clip coefficient in binary32 and rounded to its tensor's dtype, in place; returns the total norm.  Nothing is
     written when nothing is clipped.  The tensors must not share memory."""
-    lst = _native.TensorList(grads, "grads", _resolve)
-    norm_and_coef = _native.list_clip(lst, norm_type, max_norm)
-    lst.bump_versions()
-    return norm_and_coef[0]
+    return _native.list_clip(grads, norm_type, max_norm, "grads", _resolve)[0]
 
 
 def list_adamw_step(
@@ -356,13 +353,11 @@ def list_adamw_step(
     _check_hyperparameters(lr, betas, eps, weight_decay)
     if step < 1:
         raise ValueError(f"Invalid step: {step}")
-    lst = _native.AdamwList(params, grads, exp_avgs, exp_avg_sqs, outs16, _resolve)
     _native.list_adamw(
-        lst, lr=lr, beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, step=step,
-        decoupled=decoupled_weight_decay, grad_scale=None if grad_scale is None else grad_scale.detach().view(1),
-        zero_grad=zero_grad,
+        params, grads, exp_avgs, exp_avg_sqs, outs16, _resolve, lr=lr, beta1=betas[0], beta2=betas[1], eps=eps,
+        weight_decay=weight_decay, step=step, decoupled=decoupled_weight_decay,
+        grad_scale=None if grad_scale is None else grad_scale.detach().view(1), zero_grad=zero_grad,
     )
-    lst.bump_versions(zero_grad)
 
 
 class _Unit:
@@ -507,9 +502,10 @@ class FlatAdamW(torch.optim.Optimizer):
             unit.steps[0] += 1
             runs.setdefault((unit.device, unit.steps[0]), []).append((unit, p, grad))
         for (_, step), run in runs.items():
-            lst = _native.AdamwList([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
-                                    [u.exp_avg_sq for u, _, _ in run], None, _resolve)
-            if _native.list_adamw(lst, step=step, grad_scale=grad_scale, zero_grad=zero_grad, allow_overlap=True, **hyper):
+            lists = ([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
+                     [u.exp_avg_sq for u, _, _ in run])
+            if _native.list_adamw(*lists, None, _resolve, step=step, grad_scale=grad_scale, zero_grad=zero_grad,
+                                  bump_versions=False, allow_overlap=True, **hyper):
                 continue
             # parameters (or zero-filled gradients) that share memory: one after the other, in the list's order
             for unit, p, grad in run:
