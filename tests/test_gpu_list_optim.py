@@ -807,6 +807,37 @@ def test_model_with_sharded_and_plain_parameters():
         torch.equal(t, torch.zeros(5, device=DEV)) for t in results[0])
 
 
+def test_adamw_list_step_on_sharded_parameters():
+    """list_adamw_step on a wrapped model's fragments: FlatAdamW's bits, and the next forward casts the new masters."""
+    from yafsdp_amd import MixedPrecisionPolicy, fully_shard
+    from yafsdp_amd.optim import FlatAdamW, list_adamw_step
+
+    torch.manual_seed(53)
+    model0 = _Net().inner.to(DEV)
+    x = torch.randn(16, 64, device=DEV)
+    outs = []
+    for with_list in (True, False):
+        model = copy.deepcopy(model0)
+        fully_shard(model, mesh=(1, 0), mp_policy=MixedPrecisionPolicy(param_dtype=BF16, cast_forward_inputs=True))
+        params = list(model.parameters())
+        opt = FlatAdamW(params, **HP)
+        state = [[torch.zeros_like(p._local_tensor.detach()) for p in params] for _ in range(2)]
+        ys = []
+        for step in range(1, 4):
+            y = model(x)
+            ys.append(y.detach().clone())
+            y.float().pow(2).mean().backward()
+            if with_list:
+                list_adamw_step(params, [p.grad for p in params], *state, step=step, zero_grad=True, **HP)
+            else:
+                opt.step()
+            opt.zero_grad(set_to_none=True)
+        ys.append(model(x).detach().clone())
+        outs.append(ys + [p._local_tensor.detach().clone() for p in params])
+    for a, b in zip(*outs):
+        assert_bits_equal(a, b, "list step == flat step")
+
+
 def test_clipping_a_sharded_gradient_makes_its_fused_norm_stale():
     from yafsdp_amd import MixedPrecisionPolicy, fully_shard
     from yafsdp_amd.optim import disable_fused_grad_norm, enable_fused_grad_norm, grad_clip_coef, list_clip_grad_norm_

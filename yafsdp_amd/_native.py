@@ -973,6 +973,13 @@ def _as_list(tensors, what: str) -> list:
     return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
 
 
+def _as_given_and_resolved(tensors, resolve):
+    """The list, then (if there is a ``resolve``) the list of what it makes of each tensor."""
+    yield tensors
+    if resolve is not None:
+        yield [None if t is None else resolve(t) for t in tensors]
+
+
 class TensorList:
     """A list of tensors as the ``yafsdp_list_*`` entry points take it: one entry per tensor, ``None`` left out.  Any
     mixture of the path's dtypes, any sizes (0 included), on one GPU; each tensor dense (contiguous in some order of
@@ -982,16 +989,14 @@ class TensorList:
     __slots__ = ("tensors", "entries", "count", "device")
 
     def __init__(self, tensors, what: str = "tensors", resolve=None):
-        tensors = _as_list(tensors, what)
-        got = _tensorlist.list_entries(tensors, True) if _tensorlist is not None else None
-        if got is not None:
-            self.tensors = tensors
-            self.entries, self.count, index = got
-            self.device = _cuda_device(index)
-            return
-        # not accepted as it stands: resolve wrappers, find out what is wrong and raise
-        if resolve is not None:
-            tensors = [None if t is None else resolve(t) for t in tensors]
+        for tensors in _as_given_and_resolved(_as_list(tensors, what), resolve):
+            got = _tensorlist.list_entries(tensors, True) if _tensorlist is not None else None
+            if got is not None:
+                self.tensors = tensors
+                self.entries, self.count, index = got
+                self.device = _cuda_device(index)
+                return
+        # not accepted as it stands: find out what is wrong and raise
         rows, device = [], None
         for i, t in enumerate(tensors):
             if t is None:
@@ -1098,14 +1103,13 @@ class AdamwList:
     def __init__(self, params, grads, exp_avgs, exp_avg_sqs, outs16=None, resolve=None):
         lists = [_as_list(ts, name) for ts, name in zip((params, grads, exp_avgs, exp_avg_sqs), self._NAMES)]
         lists.append(None if outs16 is None else _as_list(outs16, "outs16"))
-        got = _tensorlist.adamw_entries(*lists, True) if _tensorlist is not None else None
-        if got is not None:
-            self.lists = lists
-            self.entries, self.count, index, self.grad_code, self.out_code = got
-            self.device = _cuda_device(index)
-            return
-        if resolve is not None:
-            lists = [None if ts is None else [None if t is None else resolve(t) for t in ts] for ts in lists]
+        for lists in zip(*([None, None] if ts is None else _as_given_and_resolved(ts, resolve) for ts in lists)):
+            got = _tensorlist.adamw_entries(*lists, True) if _tensorlist is not None else None
+            if got is not None:
+                self.lists = lists
+                self.entries, self.count, index, self.grad_code, self.out_code = got
+                self.device = _cuda_device(index)
+                return
         n = len(lists[0])
         for ts, name in zip(lists, self._NAMES):
             if ts is not None and len(ts) != n:
