@@ -396,7 +396,7 @@ int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_
  * in any mixture of the three dtypes.  The reference runs these as torch foreach
  * ops over the list (torch.nn.utils.clip_grad_norm_, ya_fsdp/_tensor.py:220-262;
  * _fused_adamw_, :300-312).  The list is a host array that the call is done with
- * when it returns.  It reaches the GPU in kernel arguments (240 ranges fit in
+ * when it returns.  It reaches the GPU in kernel arguments (320 ranges fit in
  * one launch, 80 of AdamW; longer lists are written to the workspace by small
  * launches first; tensors that follow each other in memory count as one range),
  * so a call keeps no state, copies nothing from host memory, may run next to any

@@ -42,7 +42,7 @@ def test_norm_and_clip_refusals(clip):
     assert _norm(one, workspace=0x10008, clip=clip) == MISALIGNED
     assert _norm(one, out=0x20002, clip=clip) == MISALIGNED
     assert _norm(one, n=-1, clip=clip) == INVALID
-    many = _entries(*[(0x100000 + 0x100 * i, 4, F32) for i in range(241)])
+    many = _entries(*[(0x100000 + 0x100 * i, 4, F32) for i in range(321)])
     assert _norm(many, clip=clip) == INVALID  # a longer list needs a larger workspace
     assert _norm((None, 1), clip=clip) == INVALID
     assert _norm(_entries((0x1000, 4, 3)), clip=clip) == DTYPE
@@ -52,6 +52,7 @@ def test_norm_and_clip_refusals(clip):
     assert _norm(_entries((0x1000, 4, F32), (0x2002, 4, F32)), clip=clip) == MISALIGNED
     assert _norm(_entries((0x2001, 4, BF16)), clip=clip) == MISALIGNED
     assert _norm(_entries((0x1000, 1 << 47, F32)), clip=clip) == TOO_LARGE
+    assert _norm(_entries((1 << 48, 4, F32)), clip=clip) == INVALID  # no device address
     # 2^45 bytes in one tensor are more tiles than one launch counts
     assert _norm(_entries((0x1000, 1 << 44, BF16)), clip=clip) == TOO_LARGE
 
@@ -238,12 +239,12 @@ def test_bump_versions_matches_torch():
 
 
 def test_workspace_sizes():
-    """Partial sums, and behind them (AdamW: alone) lists that the kernel arguments do not hold: 4 (12) words per entry in
+    """Partial sums, and behind them (AdamW: alone) lists that the kernel arguments do not hold: 3 (12) words per entry in
     whole pieces of 960."""
     norm, adamw = _native.lib.yafsdp_list_workspace_bytes, _native.lib.yafsdp_list_adamw_workspace_bytes
-    assert norm(0) == norm(240) == 1024 * 8
-    for n in (241, 480, 481, 5000):
-        assert norm(n) == norm(0) + -(-4 * n // 960) * 960 * 4
+    assert norm(0) == norm(320) == 1024 * 8
+    for n in (321, 640, 641, 5000):
+        assert norm(n) == norm(0) + -(-3 * n // 960) * 960 * 4
     assert adamw(0) == adamw(80) == 0
     for n in (81, 160, 161, 3000):
         assert adamw(n) == -(-12 * n // 960) * 960 * 4

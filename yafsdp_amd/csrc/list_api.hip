@@ -66,6 +66,7 @@ int collect(const yafsdp_list_entry* entries, int64_t n, std::vector<Range>& out
     if (!aligned_to(e.data, size)) return YAFSDP_ERR_MISALIGNED;
     const uintptr_t addr = reinterpret_cast<uintptr_t>(e.data);
     const uint64_t bytes = uint64_t(e.numel) * size;
+    if (addr >> kListAddrBits != 0) return YAFSDP_ERR_INVALID_ARGUMENT;  // no device address
     int& l = last[e.dtype];
     if (l >= 0 && out[l].addr + out[l].bytes == addr) {
       out[l].bytes += bytes;
@@ -93,6 +94,11 @@ int grid_of(uint32_t n_tiles, int block, int cap) {
 
 constexpr size_t kPartialBytes = size_t(kListNormGrid) * sizeof(double);
 constexpr size_t kAdamRecordWords = sizeof(ListAdamRange) / sizeof(uint32_t);
+static_assert((kAdamRecordWords + 2) % 4 == 0, "whole 16-byte vectors");
+
+// 32-bit words of a staged list of n ranges: whole 16-byte vectors.
+size_t list_words(size_t n) { return (3 * n + 3) / 4 * 4; }
+size_t adam_words(size_t n) { return (kAdamRecordWords + 2) * n; }
 
 // Bytes of `words` 32-bit words in the workspace: whole pieces of kListStageWords.
 size_t staged_bytes(size_t words) {
@@ -171,37 +177,36 @@ struct Tiles {
 };
 
 // Where range r lies in tiles counted from the 128-byte line that holds its first element.
-bool cut(const Range& r, Tiles& tiles, uint32_t* tile_end, uint32_t* tail) {
+bool cut(const Range& r, Tiles& tiles, uint32_t* tile_end, uint64_t* word) {
   const uint64_t end = (r.addr & 127) + r.bytes, n = (end + kListTileBytes - 1) / kListTileBytes;
   if (!tiles.add(n)) return false;
   *tile_end = uint32_t(tiles.count);
-  *tail = uint32_t(end - (n - 1) * kListTileBytes) | uint32_t(r.dtype) << 30;
+  *word = list_word(r.addr, uint32_t(end - (n - 1) * kListTileBytes), r.dtype);
   return true;
 }
+static_assert(kListTileBytes == 1 << kListTailBits, "the end inside a tile, minus one, has kListTailBits bits");
 
 int pack(const std::vector<Range>& ranges, ListArgs& a) {
   Tiles tiles;
   a.n = int32_t(ranges.size());
-  for (int k = 0; k < a.n; k++) {
-    if (!cut(ranges[k], tiles, &a.tile_end[k], &a.tail[k])) return YAFSDP_ERR_TOO_LARGE;
-    a.addr[k] = ranges[k].addr;
-  }
+  for (int k = 0; k < a.n; k++)
+    if (!cut(ranges[k], tiles, &a.tile_end[k], &a.range[k])) return YAFSDP_ERR_TOO_LARGE;
   a.n_tiles = uint32_t(tiles.count);
   return YAFSDP_OK;
 }
 
-// The list behind the partial sums of the workspace: addresses, then the two word arrays.
+// The list behind the partial sums of the workspace: the ranges, then where their tiles end.
 int pack_and_stage(const std::vector<Range>& ranges, void* workspace, hipStream_t stream, ListRef& a) {
   const size_t n = ranges.size();
-  std::vector<uint32_t> words(4 * n);
+  std::vector<uint32_t> words(list_words(n));
   Tiles tiles;
   for (size_t k = 0; k < n; k++) {
-    words[2 * k] = uint32_t(ranges[k].addr);
-    words[2 * k + 1] = uint32_t(uint64_t(ranges[k].addr) >> 32);
-    if (!cut(ranges[k], tiles, &words[2 * n + k], &words[3 * n + k])) return YAFSDP_ERR_TOO_LARGE;
+    uint64_t word;
+    if (!cut(ranges[k], tiles, &words[2 * n + k], &word)) return YAFSDP_ERR_TOO_LARGE;
+    std::memcpy(&words[2 * k], &word, sizeof(word));
   }
   uint32_t* base = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kPartialBytes);
-  a = ListRef{int32_t(n), uint32_t(tiles.count), base + 2 * n, base + 3 * n, reinterpret_cast<const uint64_t*>(base)};
+  a = ListRef{int32_t(n), uint32_t(tiles.count), base + 2 * n, reinterpret_cast<const uint64_t*>(base)};
   return stage(words, base, stream);
 }
 
@@ -257,11 +262,11 @@ int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double m
 extern "C" {
 
 size_t yafsdp_list_workspace_bytes(int64_t n) {
-  return kPartialBytes + (n > kListMax ? staged_bytes(size_t(n) * 4) : 0);
+  return kPartialBytes + (n > kListMax ? staged_bytes(list_words(size_t(n))) : 0);
 }
 
 size_t yafsdp_list_adamw_workspace_bytes(int64_t n) {
-  return n > kListAdamMax ? staged_bytes(size_t(n) * (kAdamRecordWords + 2)) : 0;
+  return n > kListAdamMax ? staged_bytes(adam_words(size_t(n))) : 0;
 }
 
 int yafsdp_list_norm(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
@@ -381,7 +386,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
     }
     return int(launch_list_adamw(grad_dtype, out16_dtype, a, s, grad_scale, stream));
   }
-  std::vector<uint32_t> words((kAdamRecordWords + 2) * k);
+  std::vector<uint32_t> words(adam_words(k));
   for (size_t i = 0; i < k; i++) {
     const ListAdamRange r = record(i);
     std::memcpy(&words[kAdamRecordWords * i], &r, sizeof(r));

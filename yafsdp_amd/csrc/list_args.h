@@ -15,21 +15,26 @@ namespace yafsdp {
 // A range's tiles start at the 128-byte line that holds its first element, so every 16-byte access is aligned and no
 // cache line is shared by two tiles of one range.
 constexpr int kListTileBytes = 4096;
-constexpr int kListMax = 240;
+constexpr int kListMax = 320;
+
+// A range in 64 bits: where its first element lies (48 bits: device addresses are below 2^47), the end of the range inside
+// its last tile minus one (12 bits) and its dtype.
+constexpr int kListAddrBits = 48, kListTailBits = 12;
+constexpr uint64_t list_word(uint64_t addr, uint32_t tail, int dtype) {
+  return addr | uint64_t(tail - 1) << kListAddrBits | uint64_t(dtype) << (kListAddrBits + kListTailBits);
+}
 
 struct ListArgs {
   int32_t n;                    // ranges
   uint32_t n_tiles;             // of all of them
   uint32_t tile_end[kListMax];  // tiles up to and including this range's
-  uint32_t tail[kListMax];      // bits 0-12: end of the range inside its last tile (1 .. 4096 bytes); bits 30-31: dtype
-  uint64_t addr[kListMax];      // first element
+  uint64_t range[kListMax];     // list_word
 };
 struct ListRef {  // the same in the workspace
   int32_t n;
   uint32_t n_tiles;
   const uint32_t* tile_end;
-  const uint32_t* tail;
-  const uint64_t* addr;
+  const uint64_t* range;
 };
 
 // ---- AdamW: one wave per tile of 256 elements ---------------------------------------------------------

@@ -27,8 +27,7 @@ __device__ __forceinline__ uint32_t global_wave() {
 // first parameter of the kernel) or from the workspace.
 struct ListView {
   const YAFSDP_CONST_AS uint32_t* tile_end;
-  const YAFSDP_CONST_AS uint32_t* tail;
-  const YAFSDP_CONST_AS uint64_t* addr;
+  const YAFSDP_CONST_AS uint64_t* range;
   int n;
   uint32_t n_tiles;
 };
@@ -50,10 +49,10 @@ __device__ __forceinline__ const YAFSDP_CONST_AS ARGS* first_argument() {
 }
 __device__ __forceinline__ ListView list_view(const ListArgs&) {
   const YAFSDP_CONST_AS ListArgs* a = first_argument<ListArgs>();
-  return ListView{a->tile_end, a->tail, a->addr, a->n, a->n_tiles};
+  return ListView{a->tile_end, a->range, a->n, a->n_tiles};
 }
 __device__ __forceinline__ ListView list_view(const ListRef& a) {
-  return ListView{as_const(a.tile_end), as_const(a.tail), as_const(a.addr), a.n, a.n_tiles};
+  return ListView{as_const(a.tile_end), as_const(a.range), a.n, a.n_tiles};
 }
 __device__ __forceinline__ ListAdamView list_view(const ListAdamArgs&) {
   const YAFSDP_CONST_AS ListAdamArgs* a = first_argument<ListAdamArgs>();
@@ -104,13 +103,15 @@ struct ListTile {
   int dtype;
 };
 
-// Tile t of range k, whose tiles are [begin, end).
-__device__ __forceinline__ ListTile tile_of(uint64_t addr, uint32_t tail, uint32_t begin, uint32_t end, uint32_t t) {
+// Tile t of a range (list_word) whose tiles are [begin, end).
+__device__ __forceinline__ ListTile tile_of(uint64_t range, uint32_t begin, uint32_t end, uint32_t t) {
+  const uint64_t addr = range & ((uint64_t(1) << kListAddrBits) - 1);
+  const uint32_t rest = uint32_t(range >> kListAddrBits);
   ListTile x;
   x.base = (addr & ~uint64_t(127)) + uint64_t(t - begin) * kListTileBytes;
   x.lo = t == begin ? int(addr & 127) : 0;
-  x.hi = t + 1 == end ? int(tail & 0x1FFFu) : kListTileBytes;
-  x.dtype = int(tail >> 30);
+  x.hi = t + 1 == end ? int(rest & ((1u << kListTailBits) - 1)) + 1 : kListTileBytes;
+  x.dtype = int(rest >> kListTailBits);
   return x;
 }
 
@@ -118,8 +119,8 @@ __device__ __forceinline__ ListTile tile_of(uint64_t addr, uint32_t tail, uint32
 struct TileCursor {
   const ListView& a;
   int k;
-  uint32_t begin, end, tail;
-  uint64_t addr;
+  uint32_t begin, end;
+  uint64_t range;
 
   __device__ __forceinline__ explicit TileCursor(const ListView& view) : a(view), k(-1), begin(0), end(0) {}
   __device__ __forceinline__ ListTile tile(uint32_t t) {
@@ -127,10 +128,9 @@ struct TileCursor {
       k = find_range(a, t, k + 1);
       begin = k > 0 ? a.tile_end[k - 1] : 0;
       end = a.tile_end[k];
-      tail = a.tail[k];
-      addr = a.addr[k];
+      range = a.range[k];
     }
-    return tile_of(addr, tail, begin, end, t);
+    return tile_of(range, begin, end, t);
   }
 };
 
@@ -417,9 +417,9 @@ __global__ void __launch_bounds__(BLOCK) list_small_kernel(ListArgs, float max_n
   const uint32_t n_tiles = a->n_tiles;
   const int i = threadIdx.x;
   if (i < a->n) {
-    const uint32_t begin = i > 0 ? a->tile_end[i - 1] : 0, end = a->tile_end[i], tail = a->tail[i];
-    const uint64_t addr = a->addr[i];
-    for (uint32_t t = begin; t < end; t++) tiles[t] = tile_of(addr, tail, begin, end, t);
+    const uint32_t begin = i > 0 ? a->tile_end[i - 1] : 0, end = a->tile_end[i];
+    const uint64_t range = a->range[i];
+    for (uint32_t t = begin; t < end; t++) tiles[t] = tile_of(range, begin, end, t);
   }
   __syncthreads();
   const uint32_t wave = global_wave<BLOCK>(), rest = wave + kHeld * kWaves;

@@ -19,7 +19,7 @@ class StageSlots {
  public:
   static constexpr int kSlots = 16;
   static constexpr size_t kPieceBytes = 16384;  // one workgroup's share: 16 bytes for each of 1024 lanes
-  static constexpr int kPieces = 32;            // of one slot at most (512 KiB: 32,768 ranges, 10,922 of AdamW)
+  static constexpr int kPieces = 32;            // of one slot at most (512 KiB: 43,690 ranges, 10,922 of AdamW)
   static constexpr size_t kSlotBytes = kPieceBytes * kPieces;
   static constexpr size_t kBlockBytes = kSlots * kSlotBytes + kSlots * kPieces * sizeof(uint32_t);
 
