@@ -258,15 +258,44 @@ def test_clip_of_neighbours_of_other_dtypes(order):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_clip_of_special_values(dtype):
     """Subnormals, signed zeros, ties: x * c in binary32, rounded once."""
-    from yafsdp_amd import _native
+    from yafsdp_amd.optim import list_scale_grads_
 
     x = mixed_values(torch.Generator().manual_seed(6), 5000, dtype)
     for c in (0.3, 0.5, 0.0, -0.7, 1e-30, 3e38, INF, float("nan"), 1.0):
         dev, want = x.to(DEV), x.clone()
         coef = torch.tensor([c], dtype=F32)
-        _native.list_scale(_native.TensorList([dev[:1234], dev[1234:]]), coef.to(DEV))
+        list_scale_grads_([dev[:1234], None, dev[1234:]], coef.to(DEV))
         cref.flat_scale(want, float(coef))
         assert_bits_equal(dev, want, f"scale by {c}")
+
+
+def test_scale_with_a_coefficient_from_elsewhere():
+    """Norms of two lists joined outside (as those of several ranks are), the lists scaled by the common coefficient:
+    the bits of clipping them as one list.  Long lists, sharded ones and refusals included."""
+    from yafsdp_amd.optim import list_clip_coef, list_clip_grad_norm_, list_scale_grads_
+
+    gen = torch.Generator().manual_seed(16)
+    cpu = [torch.randn(n, generator=gen).to(DTYPES[i % 3]) for i, n in enumerate([5, 3000, 77, 1] + [9] * 400)]
+    a, b = [t.to(DEV) for t in cpu], [t.to(DEV) for t in cpu]
+    norm, coef = list_clip_coef(a, 1.0)
+    parts = [list_clip_coef(a[:7], 1.0)[0], list_clip_coef(a[7:], 1.0)[0]]
+    joined = torch.stack(parts).double().pow(2).sum().sqrt().float()
+    assert abs(joined.item() - norm.item()) <= 2 * 2.0 ** -24 * norm.item()
+    version = a[0]._version
+    list_scale_grads_(a[:7], coef)
+    list_scale_grads_(a[7:], coef)
+    assert a[0]._version == version + 1
+    list_clip_grad_norm_(b, 1.0)
+    for x, y in zip(a, b):
+        assert_bits_equal(x, y, "scaled in two lists, clipped as one")
+    before = a[1].clone()
+    with pytest.raises(RuntimeError, match="share memory"):
+        list_scale_grads_([a[1], a[1][5:]], coef)
+    with pytest.raises(TypeError, match="coef"):
+        list_scale_grads_(a, coef.double())
+    with pytest.raises(RuntimeError, match="coef must live on the GPU"):
+        list_scale_grads_(a, torch.ones(1))
+    assert_bits_equal(a[1], before, "a refused call writes nothing")
 
 
 def test_clip_of_nonfinite_gradients_follows_torch():

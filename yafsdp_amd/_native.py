@@ -1079,17 +1079,20 @@ def list_clip(tensors, norm_type, max_norm: float, what: str = "tensors", resolv
     return norm_and_coef
 
 
-def list_scale(lst: TensorList, coef: torch.Tensor) -> None:
-    """``t.mul_(coef)`` for every tensor of the list, ``coef`` a one-element float32 device tensor."""
+def list_scale(tensors, coef: torch.Tensor, what: str = "tensors", resolve=None) -> None:
+    """``t.mul_(coef)`` for every tensor of a list (see ``TensorList``), ``coef`` a one-element float32 device tensor."""
     _flat_arg(coef, "coef")
+    lst = TensorList(tensors, what, resolve)
     if coef.dtype != torch.float32 or coef.numel() != 1 or coef.device != lst.device:
         raise TypeError("coef must be a one-element float32 tensor on the list's device")
     workspace, nbytes = _list_workspace(lst)
     with _on(lst.device):
         _check(
-            lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), workspace.data_ptr(), nbytes, _stream(coef)),
+            lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), workspace.data_ptr(), nbytes,
+                                  _device_stream(lst.device)),
             "yafsdp_list_scale",
         )
+    _bump_versions(lst.tensors)
 
 
 class AdamwList:

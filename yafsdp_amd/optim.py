@@ -29,6 +29,7 @@ torch                                          here
 ``torch.nn.utils.get_total_norm``              ``list_grad_norm``
 norm + clip coefficient, gradients untouched   ``list_clip_coef``
 ``torch.nn.utils.clip_grad_norm_``             ``list_clip_grad_norm_``
+``clip_grads_with_norm_``, coefficient known   ``list_scale_grads_``
 functional ``adamw`` over parallel lists       ``list_adamw_step``
 =============================================  ==============================
 
@@ -52,7 +53,7 @@ from ._state import _get_module_fsdp_state
 
 __all__ = ["FlatAdamW", "clip_grad_norm_", "grad_clip_coef", "zero_grad", "fsdp_param_groups",
            "enable_fused_grad_norm", "disable_fused_grad_norm", "list_grad_norm", "list_clip_coef",
-           "list_clip_grad_norm_", "list_adamw_step"]
+           "list_clip_grad_norm_", "list_scale_grads_", "list_adamw_step"]
 
 
 def fsdp_param_groups(modules: nn.Module | Iterable[nn.Module]) -> list[YaFSDPParamGroup]:
@@ -323,6 +324,14 @@ def list_clip_grad_norm_(
     by the clip coefficient in binary32 and rounded to its tensor's dtype, in place; returns the total norm.  Nothing is
     written when nothing is clipped.  The tensors must not share memory."""
     return _native.list_clip(grads, norm_type, max_norm, "grads", _resolve)[0]
+
+
+def list_scale_grads_(grads: Iterable[torch.Tensor | None], coef: torch.Tensor) -> None:
+    """Every gradient of the list (see ``list_clip_coef``) times ``coef``, a one-element float32 device tensor, in place:
+    the second half of ``list_clip_grad_norm_`` for a coefficient that comes from elsewhere, for instance from the norms
+    of all ranks.  The product is rounded to each tensor's dtype; nothing is written when ``coef`` is exactly 1.  The
+    tensors must not share memory."""
+    _native.list_scale(grads, coef.detach().view(1), "grads", _resolve)
 
 
 def list_adamw_step(
