@@ -397,16 +397,20 @@ int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_
  * ops over the list (torch.nn.utils.clip_grad_norm_, ya_fsdp/_tensor.py:220-262;
  * _fused_adamw_, :300-312).  The list is a host array that the call is done with
  * when it returns.  It reaches the GPU in kernel arguments (320 ranges fit in
- * one launch, 80 of AdamW; longer lists are written to the workspace by small
- * launches first; tensors that follow each other in memory count as one range),
- * so a call keeps no state, copies nothing from host memory, may run next to any
- * other on any stream, and can be captured into a HIP graph (which then holds
- * the addresses).  `workspace` (16-byte aligned device memory) is scratch for the
- * duration of the call on `stream` and needs no particular contents; its size is
- * a function of the number of entries.  Entries with numel 0 are skipped
- * whatever their pointer.  Data is element-aligned; any such address works,
- * 128-byte aligned starts are fastest.  Lists of 2^31 tiles (8 TB; 2^39
- * elements for AdamW) or more are refused (YAFSDP_ERR_TOO_LARGE). */
+ * one launch, 80 of AdamW; tensors that follow each other in memory count as
+ * one range).  A longer list is written to the workspace by a small launch in
+ * front, from one of 16 pinned staging slots of the library (8 MiB, allocated by
+ * the first such call and held until the process ends); while every slot is
+ * still unread, for a list longer than a slot, and under graph capture, several
+ * launches carry it in their arguments instead.  No call waits or keeps anything
+ * for the next: calls may run at once on any streams, and can be captured into
+ * a HIP graph (which then holds the addresses).  `workspace` (16-byte aligned
+ * device memory) is scratch for the duration of the call on `stream` and needs
+ * no particular contents; its size is a function of the number of entries.
+ * Entries with numel 0 are skipped whatever their pointer.  Data is
+ * element-aligned; any such address works, 128-byte aligned starts are fastest.
+ * Lists of 2^31 tiles (8 TB; 2^39 elements for AdamW) or more are refused
+ * (YAFSDP_ERR_TOO_LARGE). */
 typedef struct yafsdp_list_entry {
   void* data; /* device pointer; only read by yafsdp_list_norm */
   int64_t numel;

@@ -416,7 +416,8 @@ class FlatAdamW(torch.optim.Optimizer):
     flat float32 shard (parameters, gradients and both moments are flat buffers
     of the shard's size), which also writes the 16-bit all-gather input of the
     next iteration, so that the copy-in cast of the next forward
-    (ya_fsdp/_collectives.py:47-55) is already done.
+    (ya_fsdp/_collectives.py:47-55) is already done.  Parameters outside any
+    group take one list pass per GPU and step count.
 
     ``params`` is what ``torch.optim.AdamW`` takes (``model.parameters()`` after
     ``fully_shard``, or param-group dicts).  ``state[p]`` holds ``exp_avg`` /
