@@ -42,6 +42,9 @@ class StageSlots {
       *number = number_;
       last_[s] = number_;
       pieces_[s] = pieces(bytes);
+      // no kernel is left that would store here; a word of an older, longer use may not pass for this number once the
+      // numbers have wrapped
+      for (int p = 0; p < pieces_[s]; p++) done(s)[p].store(0, std::memory_order_relaxed);
       return s;
     }
     return -1;
