@@ -435,12 +435,14 @@ int yafsdp_list_norm(const yafsdp_list_entry* entries, int64_t n, int norm, doub
                      size_t workspace_bytes, float* norm_and_coef, void* stream);
 
 /* yafsdp_list_norm followed by x = round(float(x) * norm_and_coef[1]) on every element, in place (nothing is
- * written when the coefficient is exactly 1).  Entries must not share memory (YAFSDP_ERR_OVERLAP, nothing launched). */
+ * written when the coefficient is exactly 1).  Entries must not share memory with each other or with norm_and_coef
+ * (YAFSDP_ERR_OVERLAP, nothing launched). */
 int yafsdp_list_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
                      size_t workspace_bytes, float* norm_and_coef, void* stream);
 
 /* x = round(float(x) * *coef) on every element, in place, the coefficient read on the device (yafsdp_flat_scale over
- * a list).  Entries must not share memory (YAFSDP_ERR_OVERLAP, nothing launched). */
+ * a list).  Entries must not share memory with each other or with the coefficient (YAFSDP_ERR_OVERLAP, nothing
+ * launched). */
 int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* workspace,
                       size_t workspace_bytes, void* stream);
 
@@ -448,7 +450,7 @@ int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* 
  * dtypes (`grad_dtype`; a 16-bit gradient is used as the binary32 number it stands for) and no alignment rule beyond
  * the element's.  `out16_dtype` YAFSDP_F32: no 16-bit copy, `out16` ignored.  param, exp_avg and exp_avg_sq are
  * binary32.  What is written (with YAFSDP_ADAM_ZERO_GRAD that includes the gradients) must not share memory with
- * anything else of the list (YAFSDP_ERR_OVERLAP, nothing launched). */
+ * anything else of the list or with *grad_scale (YAFSDP_ERR_OVERLAP, nothing launched). */
 typedef struct yafsdp_adamw_entry {
   float* param;
   void* grad;

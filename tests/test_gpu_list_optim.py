@@ -298,6 +298,31 @@ def test_scale_with_a_coefficient_from_elsewhere():
     assert_bits_equal(a[1], before, "a refused call writes nothing")
 
 
+def test_scalars_that_share_memory_with_the_list():
+    """Refused where the call writes them; right beside the list, or in a gradient that is only read, they are taken."""
+    from yafsdp_amd.optim import list_adamw_step, list_scale_grads_
+
+    x = torch.full((101,), 0.5, device=DEV)
+    before = x.clone()
+    for k in (0, 50, 99):
+        with pytest.raises(RuntimeError, match="share memory"):
+            list_scale_grads_([x[:100]], x[k])
+    p, m, v = (torch.ones(100, device=DEV) for _ in range(3))
+    with pytest.raises(RuntimeError, match="share memory"):
+        list_adamw_step([p], [x[:100]], [m], [v], step=1, grad_scale=x[0], zero_grad=True)
+    with pytest.raises(RuntimeError, match="share memory"):
+        list_adamw_step([p], [x[:100]], [m], [v], step=1, grad_scale=p[99])
+    assert_bits_equal(x, before, "a refused call writes nothing")
+    assert_bits_equal(p, torch.ones_like(p), "a refused call writes nothing")
+    list_scale_grads_([x[:100]], x[100])
+    assert_bits_equal(x, torch.cat([before[:100] * 0.5, before[100:]]), "scaled by its neighbour")
+    q, a, b = p.clone(), m.clone(), v.clone()
+    list_adamw_step([p], [x[:100]], [m], [v], step=1, grad_scale=x[3])
+    list_adamw_step([q], [x[:100]], [a], [b], step=1, grad_scale=x[3].clone())
+    for got, want in ((p, q), (m, a), (v, b)):
+        assert_bits_equal(got, want, "a factor inside a gradient that is only read")
+
+
 def test_clip_of_nonfinite_gradients_follows_torch():
     from yafsdp_amd.optim import list_clip_grad_norm_
 

@@ -70,6 +70,20 @@ def test_writes_to_shared_memory_are_refused(call, rows):
     assert "share memory" in _native.error_string(rc)
 
 
+def test_scalars_inside_what_is_written_are_refused():
+    """A coefficient that its own call rewrites would be read by some waves before and by others after."""
+    one = _entries((0x9000, 64, BF16), (0x1000, 64, F32))  # up to 0x9080 and 0x1100
+    for at in (0x1000, 0x10fc, 0x907c):
+        assert _scale(one, coef=at) == OVERLAP
+    for at in (0xffc, 0x10fc, 0x8ffc, 0x9000):  # two numbers, eight bytes
+        assert _norm(one, out=at, clip=True) == OVERLAP
+    row = (0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 8)
+    for k in (0, 2, 3):
+        assert _adamw(_adam(row), scale=row[k] + 28) == OVERLAP
+    assert _adamw(_adam(row), scale=0x2000, flags=_native.ADAM_ZERO_GRAD) == OVERLAP
+    assert _adamw(_adam(row), scale=0x500c, out=F16) == OVERLAP
+
+
 def test_scale_refusals_and_empty_list():
     one = _entries((0x1000, 4, F32))
     assert _scale(one, coef=None) == INVALID and _scale(one, coef=0x20001) == MISALIGNED

@@ -45,6 +45,12 @@ bool disjoint(const std::vector<Span>& s) {
     if (s[i - 1].hi > s[i].lo) return false;
   return true;
 }
+// True if one of the sorted disjoint spans shares a byte with the one given.
+bool touches(const std::vector<Span>& s, const void* data, size_t bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(data);
+  const auto it = std::lower_bound(s.begin(), s.end(), lo, [](const Span& a, uintptr_t at) { return a.hi <= at; });
+  return it != s.end() && it->lo < lo + bytes;
+}
 // Adds sorted spans to sorted spans.
 void merge_spans(std::vector<Span>& into, const std::vector<Span>& s) {
   const size_t mid = into.size();
@@ -78,12 +84,27 @@ int collect(const yafsdp_list_entry* entries, int64_t n, std::vector<Range>& out
   return YAFSDP_OK;
 }
 
-int check_disjoint(const std::vector<Range>& ranges) {
+// Tiles so far; false when a launch cannot count them.
+struct Tiles {
+  uint64_t count = 0;
+  bool add(uint64_t n) { return (count += n) <= uint64_t(INT32_MAX); }
+};
+
+// Where a range ends, and its tiles, counted from the 128-byte line that holds its first element.
+uint64_t end_of(const Range& r) { return (r.addr & 127) + r.bytes; }
+uint64_t tiles_of(const Range& r) { return (end_of(r) + kListTileBytes - 1) / kListTileBytes; }
+
+// The ranges, which are rewritten, against each other and against the scalars that the waves read meanwhile.
+int check_disjoint(const std::vector<Range>& ranges, const float* scalars, int n_scalars) {
   std::vector<Span> spans;
   spans.reserve(ranges.size());
-  for (const Range& r : ranges) spans.push_back(Span{r.addr, r.addr + r.bytes});
+  Tiles tiles;
+  for (const Range& r : ranges) {
+    if (!tiles.add(tiles_of(r))) return YAFSDP_ERR_TOO_LARGE;
+    spans.push_back(Span{r.addr, r.addr + r.bytes});
+  }
   sort_spans(spans);
-  return disjoint(spans) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
+  return disjoint(spans) && !touches(spans, scalars, n_scalars * sizeof(float)) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
 }
 
 // workgroups of `block` lanes, one wave per tile, at most `cap`
@@ -170,18 +191,12 @@ int stage(const std::vector<uint32_t>& words, void* dst, hipStream_t stream) {
 }
 static_assert(StageSlots::kPieceBytes == size_t(kListFetchBlock) * 16, "a workgroup reads a piece");
 
-// Tiles so far; false when a launch cannot count them.
-struct Tiles {
-  uint64_t count = 0;
-  bool add(uint64_t n) { return (count += n) <= uint64_t(INT32_MAX); }
-};
-
-// Where range r lies in tiles counted from the 128-byte line that holds its first element.
+// What the kernels know of range r.
 bool cut(const Range& r, Tiles& tiles, uint32_t* tile_end, uint64_t* word) {
-  const uint64_t end = (r.addr & 127) + r.bytes, n = (end + kListTileBytes - 1) / kListTileBytes;
+  const uint64_t n = tiles_of(r);
   if (!tiles.add(n)) return false;
   *tile_end = uint32_t(tiles.count);
-  *word = list_word(r.addr, uint32_t(end - (n - 1) * kListTileBytes), r.dtype);
+  *word = list_word(r.addr, uint32_t(end_of(r) - (n - 1) * kListTileBytes), r.dtype);
   return true;
 }
 static_assert(kListTileBytes == 1 << kListTailBits, "the end inside a tile, minus one, has kListTailBits bits");
@@ -246,7 +261,7 @@ int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double m
   if (!aligned_to(workspace, 16) || !aligned_to(norm_and_coef, 4)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
-  if (rc == YAFSDP_OK && clip) rc = check_disjoint(ranges);
+  if (rc == YAFSDP_OK && clip) rc = check_disjoint(ranges, norm_and_coef, 2);
   if (rc != YAFSDP_OK) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
     if constexpr (std::is_same<std::decay_t<decltype(a)>, ListArgs>::value)
@@ -293,7 +308,7 @@ int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* 
   if (!aligned_to(coef, 4) || !aligned_to(workspace, 16)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
-  if (rc == YAFSDP_OK) rc = check_disjoint(ranges);
+  if (rc == YAFSDP_OK) rc = check_disjoint(ranges, coef, 1);
   if (rc != YAFSDP_OK || ranges.empty()) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
     return int(launch_list_scale(a, coef, stream));
@@ -355,6 +370,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
   if (has_out) add(&AdamRange::out, 2, true);
   add(&AdamRange::g, gsize, zero);
   if (!disjoint(written)) return YAFSDP_ERR_OVERLAP;
+  if (grad_scale != nullptr && touches(written, grad_scale, sizeof(float))) return YAFSDP_ERR_OVERLAP;
   size_t w = 0;
   for (size_t i = 0; i < spans.size() && !zero; i++) {  // the gradients, sorted, against what is written
     while (w < written.size() && written[w].hi <= spans[i].lo) w++;

@@ -330,7 +330,7 @@ def list_scale_grads_(grads: Iterable[torch.Tensor | None], coef: torch.Tensor) 
     """Every gradient of the list (see ``list_clip_coef``) times ``coef``, a one-element float32 device tensor, in place:
     the second half of ``list_clip_grad_norm_`` for a coefficient that comes from elsewhere, for instance from the norms
     of all ranks.  The product is rounded to each tensor's dtype; nothing is written when ``coef`` is exactly 1.  The
-    tensors must not share memory."""
+    tensors must not share memory with each other or with ``coef``."""
     _native.list_scale(grads, coef.detach().view(1), "grads", _resolve)
 
 
@@ -358,7 +358,7 @@ def list_adamw_step(
     made.  ``grad_scale`` (one-element float32 device tensor, e.g. from ``list_clip_coef``) multiplies every gradient
     first, in binary32, without writing it back; ``zero_grad=True`` zero-fills the gradients in the same pass.  Per
     element the arithmetic is that of ``FlatAdamW``, bit for bit.  All tensors are contiguous, live on one GPU, and what
-    is written shares no memory with anything else in the lists."""
+    is written shares no memory with anything else in the lists or with ``grad_scale``."""
     _check_hyperparameters(lr, betas, eps, weight_decay)
     if step < 1:
         raise ValueError(f"Invalid step: {step}")
