@@ -1,0 +1,83 @@
+"""What the list passes and FlatAdamW promise around the arithmetic, on the GPU: which tensors they take for what."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+from ext_subclasses import Int8Master
+from helpers import assert_bits_equal
+from list_subclasses import OwnStorage, PairTensor
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+F32 = torch.float32
+HP = dict(lr=1e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+# ---- tensor subclasses -----------------------------------------------------------------------------------------
+def test_wrappers_from_elsewhere_are_refused_and_left_alone():
+    from yafsdp_amd.optim import FlatAdamW, list_adamw_step, list_clip_grad_norm_, list_scale_grads_
+
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    halves = [torch.randn(100, device=DEV, generator=gen) for _ in range(4)]
+    before = [t.clone() for t in halves]
+    p, g = nn.Parameter(PairTensor(*halves[:2])), PairTensor(*halves[2:])
+    p.grad = g
+    plain = nn.Parameter(torch.ones(7, device=DEV))
+    plain.grad = torch.ones(7, device=DEV)
+    m, v = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    opt = FlatAdamW([plain, p], **HP)
+    for call in (lambda: list_clip_grad_norm_([plain.grad, g], 1e-3),
+                 lambda: list_scale_grads_([g], torch.full((1,), 0.5, device=DEV)),
+                 lambda: list_adamw_step([p], [g], [m], [v], step=1), lambda: opt.step()):
+        with pytest.raises(TypeError, match="PairTensor keeps its values in other tensors"):
+            call()
+    for t, b in zip(halves, before):
+        assert_bits_equal(t, b, "a refused call writes nothing")
+    assert_bits_equal(plain, torch.ones(7), "nor any other tensor of its list")
+
+
+def test_subclass_with_elements_of_its_own():
+    from yafsdp_amd.optim import FlatAdamW, list_clip_grad_norm_
+
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    base, grad = (torch.randn(300, device=DEV, generator=gen) for _ in range(2))
+    out = []
+    for cls in (OwnStorage, torch.Tensor):
+        p = base.clone().as_subclass(cls).requires_grad_()
+        p.grad = grad.clone().as_subclass(cls)
+        norm = list_clip_grad_norm_([p.grad], 0.5)
+        FlatAdamW([p], **HP).step()
+        out.append([x.as_subclass(torch.Tensor).detach() for x in (norm, p.grad, p)])
+    for a, b in zip(*out):
+        assert_bits_equal(a, b, "subclass and plain tensor")
+
+
+def test_fragments_of_sharded_subclass_parameters():
+    """Parameters, gradients and states of a group whose parameters are a tensor subclass: the fragments' values."""
+    from yafsdp_amd import FSDPMeshInfo, MixedPrecisionPolicy
+    from yafsdp_amd._param_group import YaFSDPParamGroup, init_shared_state
+    from yafsdp_amd.optim import list_adamw_step, list_clip_grad_norm_
+
+    gen = torch.Generator().manual_seed(3)
+    values = [torch.randn(s, generator=gen) * 0.08 for s in ((33, 7), (5, 13), (1000,))]
+    policy = MixedPrecisionPolicy(param_dtype=torch.bfloat16, all_gather_dtype_to_param_cls={torch.int8: Int8Master})
+    group = YaFSDPParamGroup([nn.Parameter(Int8Master(v.to(DEV))) for v in values], FSDPMeshInfo(2, 1), DEV, policy, 8)
+    init_shared_state([group], DEV)
+    fps = [fp for fp in group._all_gather_dtype_to_fsdp_params[torch.int8] if fp.sharded_numel]
+    assert fps
+    for fp in fps:
+        fp.sharded_param_grad._local_tensor.copy_(torch.randn(fp.sharded_numel, generator=gen))
+    params, grads = [fp.sharded_param for fp in fps], [fp.sharded_param_grad for fp in fps]
+    plain = [[fp._sharded_param_data.clone() for fp in fps], [g._local_tensor.clone() for g in grads]]
+    states = [[torch.zeros_like(p.detach()) for p in params] for _ in range(2)]
+    assert isinstance(states[0][0]._local_tensor, Int8Master)
+    plain += [[torch.zeros_like(p) for p in plain[0]] for _ in range(2)]
+    norms = [list_clip_grad_norm_(g, 0.5) for g in (grads, plain[1])]
+    assert_bits_equal(norms[0], norms[1], "norm")
+    list_adamw_step(params, grads, *states, step=1, **HP)
+    list_adamw_step(*plain, step=1, **HP)
+    for k, fp in enumerate(fps):
+        got = (fp._sharded_param_data, grads[k]._local_tensor, *(s[k]._local_tensor._data for s in states))
+        for a, b in zip(got, (x[k] for x in plain)):
+            assert_bits_equal(a, b, f"fragment {k}")

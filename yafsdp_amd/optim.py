@@ -46,14 +46,17 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from ._param import YaFSDPParam
+from ._param import YaFSDPParam, _inner_tensor_names
 from ._param_group import YaFSDPParamGroup
-from ._tensor import local_tensor, plain_tensor
+from ._tensor import RaggedShardDTensor, local_tensor, plain_tensor
 from ._state import _get_module_fsdp_state
 
 __all__ = ["FlatAdamW", "clip_grad_norm_", "grad_clip_coef", "zero_grad", "fsdp_param_groups",
            "enable_fused_grad_norm", "disable_fused_grad_norm", "list_grad_norm", "list_clip_coef",
            "list_clip_grad_norm_", "list_scale_grads_", "list_adamw_step"]
+
+
+_PLAIN = (torch.Tensor, nn.Parameter)
 
 
 def fsdp_param_groups(modules: nn.Module | Iterable[nn.Module]) -> list[YaFSDPParamGroup]:
@@ -293,8 +296,25 @@ def _check_hyperparameters(lr, betas: tuple[float, float], eps: float, weight_de
 
 
 def _resolve(t: torch.Tensor) -> torch.Tensor:
-    """The plain tensor behind a sharded parameter or gradient: this rank's fragment."""
-    return plain_tensor(local_tensor(t)) if isinstance(t, torch.Tensor) else t
+    """The plain tensor behind a sharded parameter, gradient or state: this rank's fragment.  Any other tensor as it is.
+
+    The fragment of a tensor-subclass parameter is the first inner tensor of what the group wraps
+    (ya_fsdp/_param.py:145-152), whatever else that subclass holds.  A tensor that an op made from it is taken only where
+    there is one inner tensor: of several, none stands for all.  A subclass that is not sharded here says nothing about
+    what its inner tensors mean (halves of a value, quantised values and scales, a result still being gathered), so
+    it is refused unless its elements are its own."""
+    if not isinstance(t, torch.Tensor):
+        return t
+    if isinstance(t, RaggedShardDTensor):
+        spec, t = t._spec, t._local_tensor
+        if spec.kind == "param" and spec.owner is not None:
+            return plain_tensor(t)
+        while type(t) not in _PLAIN and len(names := _inner_tensor_names(t) or ()) == 1:
+            t = getattr(t, names[0])
+    if type(t) not in _PLAIN and t.layout == torch.strided and t.numel() and t.data_ptr() == 0:
+        raise TypeError(f"{type(t).__name__} keeps its values in other tensors and is not a sharded tensor of this "
+                        "framework: pass the plain tensors that hold them")
+    return t
 
 
 def list_clip_coef(
@@ -305,7 +325,8 @@ def list_clip_coef(
     ``FlatAdamW.step`` to fuse the scaling into the optimizer pass.
 
     ``grads`` may mix float32, bfloat16 and float16; ``None`` entries (parameters without a gradient) are left out, and
-    a sharded gradient counts with this rank's fragment.  Each is dense in memory, all live on one GPU.  ``norm_type``
+    a sharded gradient counts with this rank's fragment.  Each is dense in memory, all live on one GPU; any other tensor
+    subclass that keeps its values in inner tensors is refused.  ``norm_type``
     is 1, 2 or infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64
     and are reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls;
     the call can be captured into a HIP graph, which then reads the same addresses at every replay."""
