@@ -406,7 +406,9 @@ int yafsdp_adamw_step(float* param, float* grad, float* exp_avg, float* exp_avg_
  * for the next: calls may run at once on any streams, and can be captured into
  * a HIP graph (which then holds the addresses).  `workspace` (16-byte aligned
  * device memory) is scratch for the duration of the call on `stream` and needs
- * no particular contents; its size is a function of the number of entries.
+ * no particular contents; its size is a function of the number of entries, and
+ * that many bytes must share no memory with the entries or with a scalar that
+ * the call reads or writes (YAFSDP_ERR_OVERLAP, nothing launched).
  * Entries with numel 0 are skipped whatever their pointer.  Data is
  * element-aligned; any such address works, 128-byte aligned starts are fastest.
  * Lists of 2^31 tiles (8 TB; 2^39 elements for AdamW) or more are refused

@@ -1,13 +1,14 @@
 """What the list passes and FlatAdamW promise around the arithmetic, as far as it can be checked without a GPU: which
-tensors they take for what."""
+tensors they take for what, which memory a call may share."""
 
 import types
 import weakref
 
+import numpy as np
 import pytest
 import torch
 
-from yafsdp_amd import optim
+from yafsdp_amd import _native, optim
 from yafsdp_amd._common import FSDPMeshInfo
 from yafsdp_amd._layout import RaggedShard
 from yafsdp_amd._tensor import RaggedShardDTensor, RaggedShardSpec
@@ -69,3 +70,51 @@ def test_flat_adamw_refuses_a_wrapper_from_elsewhere():
     units = _plain_units([p], [g], [0])
     with pytest.raises(TypeError, match="keeps its values in other tensors"):
         opt._step_plain(units, HYPER, None, False)
+
+
+# ---- the workspace ---------------------------------------------------------------------------------------------
+OVERLAP = -9
+AT = 0x100000  # of the workspace; every call below is refused before anything reads its addresses
+
+
+def _norm(rows, clip, out=0x20000):
+    fn = _native.lib.yafsdp_list_clip if clip else _native.lib.yafsdp_list_norm
+    buf = np.array([(*r, 0) for r in rows], dtype=_native._LIST_ENTRY).tobytes()
+    return fn(buf, len(rows), 2, 1.0, AT, _native.lib.yafsdp_list_workspace_bytes(len(rows)) + 0x1000, out, None)
+
+
+def _scale(rows, coef=0x20000):
+    buf = np.array([(*r, 0) for r in rows], dtype=_native._LIST_ENTRY).tobytes()
+    return _native.lib.yafsdp_list_scale(buf, len(rows), coef, AT,
+                                         _native.lib.yafsdp_list_workspace_bytes(len(rows)) + 0x1000, None)
+
+
+def _adamw(rows, out=0, scale=None):
+    buf = np.array(rows, dtype=_native._ADAMW_ENTRY).tobytes()
+    return _native.lib.yafsdp_list_adamw(buf, len(rows), 1, out, 1e-3, 0.9, 0.95, 1e-8, 0.1, 1, scale, 1, AT,
+                                         _native.lib.yafsdp_list_adamw_workspace_bytes(len(rows)) + 0x1000, None)
+
+
+@pytest.mark.parametrize("count", [1, 400])  # partial sums only; with a list behind them
+def test_memory_inside_the_workspace_is_refused(count):
+    """Partial sums and staged lists are written there: a result, a coefficient or a tensor of the list would be
+    overwritten, or read half before and half after."""
+    used = _native.lib.yafsdp_list_workspace_bytes(count)
+    rows = [(0x1000000 + 0x100 * i, 4, 1) for i in range(count)]
+    for at in (AT - 4, AT, AT + 8, AT + used - 4):
+        assert _norm(rows, True, out=at) == OVERLAP and _norm(rows, False, out=at) == OVERLAP, hex(at)
+    for at in (AT, AT + 64, AT + used - 4):
+        assert _scale(rows, coef=at) == OVERLAP
+    for at, n in ((AT - 14, 8), (AT, 8), (AT + used - 2, 1), (AT - 0x1000, 0x100000)):
+        inside = [*rows[1:], (at, n, 1)]
+        assert [_norm(inside, True), _norm(inside, False), _scale(inside)] == [OVERLAP] * 3, hex(at)
+    assert "workspace" in _native.error_string(OVERLAP)
+
+
+def test_memory_inside_the_workspace_of_adamw_is_refused():
+    used = _native.lib.yafsdp_list_adamw_workspace_bytes(100)
+    rows = [tuple(0x1000000 * k + 0x100 * i for k in range(1, 6)) + (8,) for i in range(100)]
+    for at in (AT, AT + used - 4):
+        assert _adamw(rows, scale=at) == OVERLAP
+        for k in range(5):  # the gradients too, which are only read
+            assert _adamw(rows[1:] + [(*rows[0][:k], at, *rows[0][k + 1:])], out=2) == OVERLAP, k

@@ -353,7 +353,9 @@ const char* yafsdp_error_string(int code) {
     case YAFSDP_ERR_UNSUPPORTED:
       return "yafsdp: this fused entry point does not serve the dtype combination (a reduce buffer that has neither "
              "the gradients' dtype nor binary32): use the two separate entry points";
-    case YAFSDP_ERR_OVERLAP: return "yafsdp: tensors of the list that the call writes share memory";
+    case YAFSDP_ERR_OVERLAP:
+      return "yafsdp: what the call writes (tensors of the list, its workspace, its results) and other tensors of the "
+             "list or a scalar that it reads share memory";
     case YAFSDP_ERR_BUSY:
       return "yafsdp: every staging slot of this table is still in use by a queued call (more than 8 different "
              "tensor sets in flight): synchronise the stream, or bind tensor sets that persist";

@@ -94,17 +94,33 @@ struct Tiles {
 uint64_t end_of(const Range& r) { return (r.addr & 127) + r.bytes; }
 uint64_t tiles_of(const Range& r) { return (end_of(r) + kListTileBytes - 1) / kListTileBytes; }
 
-// The ranges, which are rewritten, against each other and against the scalars that the waves read meanwhile.
-int check_disjoint(const std::vector<Range>& ranges, const float* scalars, int n_scalars) {
-  std::vector<Span> spans;
-  spans.reserve(ranges.size());
+// Whether two spans share a byte.
+bool share(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+Span span_of(const void* data, size_t bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(data);
+  return Span{lo, lo + bytes};
+}
+
+// The workspace, which every call writes, against the ranges and the scalars; with `written`, the ranges (which are
+// rewritten) against each other and against the scalars that the waves read meanwhile.
+int check_memory(const std::vector<Range>& ranges, bool written, const float* scalars, int n_scalars,
+                 const void* workspace, size_t workspace_bytes) {
+  const Span scratch = span_of(workspace, workspace_bytes), scalar = span_of(scalars, n_scalars * sizeof(float));
+  bool shared = share(scratch, scalar);
   Tiles tiles;
+  std::vector<Span> spans;
+  if (written) spans.reserve(ranges.size());
   for (const Range& r : ranges) {
     if (!tiles.add(tiles_of(r))) return YAFSDP_ERR_TOO_LARGE;
-    spans.push_back(Span{r.addr, r.addr + r.bytes});
+    const Span s{r.addr, r.addr + r.bytes};
+    shared |= share(s, scratch);
+    if (!written) continue;
+    shared |= share(s, scalar);
+    spans.push_back(s);
   }
+  if (shared) return YAFSDP_ERR_OVERLAP;
   sort_spans(spans);
-  return disjoint(spans) && !touches(spans, scalars, n_scalars * sizeof(float)) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
+  return disjoint(spans) ? YAFSDP_OK : YAFSDP_ERR_OVERLAP;
 }
 
 // workgroups of `block` lanes, one wave per tile, at most `cap`
@@ -256,12 +272,13 @@ int norm_or_clip_launches(const META& a, int norm, float max_norm, double* parti
 int norm_or_clip(const yafsdp_list_entry* entries, int64_t n, int norm, double max_norm, void* workspace,
                  size_t workspace_bytes, float* norm_and_coef, hipStream_t stream, bool clip) {
   if (norm != LIST_NORM_1 && norm != LIST_NORM_2 && norm != LIST_NORM_INF) return YAFSDP_ERR_INVALID_ARGUMENT;
-  if (n < 0 || workspace == nullptr || norm_and_coef == nullptr || workspace_bytes < yafsdp_list_workspace_bytes(n))
+  const size_t need = yafsdp_list_workspace_bytes(n);
+  if (n < 0 || workspace == nullptr || norm_and_coef == nullptr || workspace_bytes < need)
     return YAFSDP_ERR_INVALID_ARGUMENT;
   if (!aligned_to(workspace, 16) || !aligned_to(norm_and_coef, 4)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
-  if (rc == YAFSDP_OK && clip) rc = check_disjoint(ranges, norm_and_coef, 2);
+  if (rc == YAFSDP_OK) rc = check_memory(ranges, clip, norm_and_coef, 2, workspace, need);
   if (rc != YAFSDP_OK) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
     if constexpr (std::is_same<std::decay_t<decltype(a)>, ListArgs>::value)
@@ -303,12 +320,12 @@ int yafsdp_list_clip(const yafsdp_list_entry* entries, int64_t n, int norm, doub
 int yafsdp_list_scale(const yafsdp_list_entry* entries, int64_t n, const float* coef, void* workspace,
                       size_t workspace_bytes, void* stream_) try {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  if (n < 0 || coef == nullptr || workspace == nullptr || workspace_bytes < yafsdp_list_workspace_bytes(n))
-    return YAFSDP_ERR_INVALID_ARGUMENT;
+  const size_t need = yafsdp_list_workspace_bytes(n);
+  if (n < 0 || coef == nullptr || workspace == nullptr || workspace_bytes < need) return YAFSDP_ERR_INVALID_ARGUMENT;
   if (!aligned_to(coef, 4) || !aligned_to(workspace, 16)) return YAFSDP_ERR_MISALIGNED;
   std::vector<Range> ranges;
   int rc = collect(entries, n, ranges);
-  if (rc == YAFSDP_OK) rc = check_disjoint(ranges, coef, 1);
+  if (rc == YAFSDP_OK) rc = check_memory(ranges, true, coef, 1, workspace, need);
   if (rc != YAFSDP_OK || ranges.empty()) return rc;
   return with_list(ranges, workspace, stream, [&](const auto& a) {
     return int(launch_list_scale(a, coef, stream));
@@ -356,7 +373,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
     }
     ranges.push_back(r);
   }
-  // what is written shares no byte with anything else; gradients that are only read may share theirs
+  // what is written (the workspace too) shares no byte with anything else; gradients that are only read may share theirs
   std::vector<Span> written, spans(ranges.size());
   const auto add = [&](uintptr_t AdamRange::*member, uint64_t size, bool is_written) {
     for (size_t i = 0; i < ranges.size(); i++)
@@ -364,6 +381,7 @@ int yafsdp_list_adamw(const yafsdp_adamw_entry* entries, int64_t n, int grad_dty
     sort_spans(spans);
     if (is_written) merge_spans(written, spans);
   };
+  if (need > 0) written.push_back(span_of(workspace, need));
   add(&AdamRange::p, 4, true);
   add(&AdamRange::m, 4, true);
   add(&AdamRange::v, 4, true);
