@@ -1,11 +1,12 @@
-"""What the list passes and FlatAdamW promise around the arithmetic, on the GPU: which tensors they take for what."""
+"""What the list passes and FlatAdamW promise around the arithmetic, on the GPU: which tensors they take for what,
+what a refused step leaves."""
 
 import pytest
 import torch
 import torch.nn as nn
 
 from ext_subclasses import Int8Master
-from helpers import assert_bits_equal
+from helpers import assert_bits_equal, loc
 from list_subclasses import OwnStorage, PairTensor
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,45 @@ def test_fragments_of_sharded_subclass_parameters():
         got = (fp._sharded_param_data, grads[k]._local_tensor, *(s[k]._local_tensor._data for s in states))
         for a, b in zip(got, (x[k] for x in plain)):
             assert_bits_equal(a, b, f"fragment {k}")
+
+
+# ---- FlatAdamW -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sharded", [False, True])
+def test_a_step_that_is_refused_can_be_made_again(sharded):
+    """Bits and counts of a run in which every step is first refused are those of a run without refusals."""
+    from yafsdp_amd import MixedPrecisionPolicy, fully_shard
+    from yafsdp_amd.optim import FlatAdamW
+
+    runs = []
+    for refused in (False, True):
+        gen = torch.Generator(device=DEV).manual_seed(5)
+        model = nn.Module()
+        for i, n in enumerate((100, 7, 2049)):
+            model.register_parameter(f"p{i}", nn.Parameter(torch.randn(n, device=DEV, generator=gen)))
+        if sharded:
+            fully_shard(model, mesh=(1, 0), mp_policy=MixedPrecisionPolicy(param_dtype=torch.bfloat16))
+        params = list(model.parameters())
+        opt = FlatAdamW(params, **HP)
+        for it in range(3):
+            for p in params[it == 1:]:
+                fresh = torch.randn(p.numel(), device=DEV, generator=gen)
+                if sharded:
+                    p.grad = p._yafsdp_param().sharded_param_grad
+                    p.grad._local_tensor.copy_(fresh)
+                else:
+                    p.grad = fresh
+            if it == 1:
+                params[0].grad = None
+            if refused:
+                before = [loc(p).detach().clone() for p in params]
+                with pytest.raises(TypeError, match="grad_scale"):
+                    opt.step(grad_scale=torch.ones(1, device=DEV, dtype=torch.float64))
+                with pytest.raises(RuntimeError, match="grad_scale"):
+                    opt.step(grad_scale=torch.ones(1))
+                for p, b in zip(params, before):
+                    assert_bits_equal(loc(p).detach(), b, "a refused step writes nothing")
+            opt.step()
+        runs.append([loc(p).detach() for p in params])
+        assert [int(s["step"]) for s in opt.state_dict()["state"].values()] == [2, 3, 3]
+    for a, b in zip(*runs):
+        assert_bits_equal(a, b, "with and without refused steps")

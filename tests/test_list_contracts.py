@@ -1,5 +1,6 @@
 """What the list passes and FlatAdamW promise around the arithmetic, as far as it can be checked without a GPU: which
-tensors they take for what, which memory a call may share."""
+tensors they take for what, which memory a call may share, what a
+refused step leaves."""
 
 import types
 import weakref
@@ -118,3 +119,34 @@ def test_memory_inside_the_workspace_of_adamw_is_refused():
         assert _adamw(rows, scale=at) == OVERLAP
         for k in range(5):  # the gradients too, which are only read
             assert _adamw(rows[1:] + [(*rows[0][:k], at, *rows[0][k + 1:])], out=2) == OVERLAP, k
+
+
+# ---- step counts -----------------------------------------------------------------------------------------------
+def test_a_refused_step_leaves_the_counts(monkeypatch):
+    """Counts advance with the launch that steps their parameters: a list at a time, or one at a time where memory is
+    shared."""
+    opt = object.__new__(optim.FlatAdamW)
+    steps = [3, 3, 0, 7]
+    params = [torch.ones(4) for _ in steps]
+
+    def refuse(*args, step, **kwargs):
+        if step == bad:
+            raise TypeError("refused")
+        return shared is None
+
+    def refuse_one(p, *args, **kwargs):
+        if p.data_ptr() == params[shared].data_ptr():
+            raise TypeError("refused")
+
+    monkeypatch.setattr(_native, "list_adamw", refuse)
+    monkeypatch.setattr(_native, "adamw_step", refuse_one)
+    for bad, shared, after in ((4, None, [3, 3, 0, 7]), (1, None, [4, 4, 0, 7]), (8, None, [4, 4, 1, 7]),
+                               (None, 0, [3, 3, 0, 7]), (None, 1, [4, 3, 0, 7]), (None, 3, [4, 4, 1, 7])):
+        units = _plain_units(params, [torch.ones(4) for _ in params], steps)
+        with pytest.raises(TypeError, match="refused"):
+            opt._step_plain(units, HYPER, None, False)
+        assert [u.steps[0] for u in units] == after, (bad, shared)
+    bad = shared = None
+    units = _plain_units(params, [torch.ones(4), None, torch.ones(4), torch.ones(4)], steps)
+    opt._step_plain(units, HYPER, None, False)
+    assert [u.steps[0] for u in units] == [4, 3, 1, 8]

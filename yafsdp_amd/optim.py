@@ -530,18 +530,21 @@ class FlatAdamW(torch.optim.Optimizer):
                 raise TypeError("FlatAdamW needs contiguous float32 gradients")
         runs: dict[tuple[torch.device, int], list[tuple[_Unit, torch.Tensor, torch.Tensor]]] = {}
         for unit, p, grad in live:
-            unit.steps[0] += 1
-            runs.setdefault((unit.device, unit.steps[0]), []).append((unit, p, grad))
+            runs.setdefault((unit.device, unit.steps[0] + 1), []).append((unit, p, grad))
         for (_, step), run in runs.items():
             lists = ([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
                      [u.exp_avg_sq for u, _, _ in run])
+            # a count advances once its launch has been accepted: what a refused call leaves can be stepped again
             if _native.list_adamw(*lists, None, _resolve, step=step, grad_scale=grad_scale, zero_grad=zero_grad,
                                   bump_versions=False, allow_overlap=True, **hyper):
+                for unit, _, _ in run:
+                    unit.steps[0] = step
                 continue
             # parameters (or zero-filled gradients) that share memory: one after the other, in the list's order
             for unit, p, grad in run:
                 _native.adamw_step(p.view(-1), grad.view(-1), unit.exp_avg, unit.exp_avg_sq, None, step=step,
                                    grad_scale=grad_scale, zero_grad=zero_grad, **hyper)
+                unit.steps[0] = step
 
     def _step_unit(self, unit: _Unit, hyper: dict[str, Any], grad_scale, zero_grad: bool) -> None:
         group = unit.group
@@ -557,9 +560,8 @@ class FlatAdamW(torch.optim.Optimizer):
         with_grad = [k for k, p in enumerate(unit.params) if p.grad is not None]
         if not with_grad:
             return
-        for k in with_grad:
-            unit.steps[k] += 1
-        uniform = len({unit.steps[k] for k in with_grad}) == 1
+        steps = {k: unit.steps[k] + 1 for k in with_grad}
+        uniform = len(set(steps.values())) == 1
         # the fused copy-in needs the whole shard rewritten in this pass; otherwise the
         # next forward casts the shard itself, as it does in the reference
         out16 = None
@@ -568,16 +570,16 @@ class FlatAdamW(torch.optim.Optimizer):
                 and group.param_dtype is not None and hasattr(group, "_all_gather_input") and group.is_sharded):
             out16 = group._all_gather_input[None]
         if whole and uniform:
-            runs = [(0, shard.numel(), unit.steps[with_grad[0]])]
+            runs = [(0, shard.numel(), steps[with_grad[0]])]
         else:
             runs = []
             for k in with_grad:
                 lo, hi = unit.fragment(k)
                 if hi > lo:
-                    if runs and runs[-1][1] == lo and runs[-1][2] == unit.steps[k]:
-                        runs[-1] = (runs[-1][0], hi, unit.steps[k])
+                    if runs and runs[-1][1] == lo and runs[-1][2] == steps[k]:
+                        runs[-1] = (runs[-1][0], hi, steps[k])
                     else:
-                        runs.append((lo, hi, unit.steps[k]))
+                        runs.append((lo, hi, steps[k]))
         if zero_grad:
             group._grad_sumsq_token.pop(key, None)  # the gradients are rewritten
         for lo, hi, step in runs:
@@ -586,6 +588,8 @@ class FlatAdamW(torch.optim.Optimizer):
                 None if out16 is None else out16[lo:hi], step=step, grad_scale=grad_scale, zero_grad=zero_grad,
                 **hyper,
             )
+        for k in with_grad:
+            unit.steps[k] = steps[k]
         if out16 is not None:
             # the next unshard finds its all-gather input ready (ya_fsdp/_collectives.py:47-55)
             for fsdp_param in class_params:
