@@ -1,5 +1,5 @@
 """What the list passes and FlatAdamW promise around the arithmetic, on the GPU: which tensors they take for what,
-what a refused step leaves."""
+what a refused step leaves, where a gradient scale may lie."""
 
 import pytest
 import torch
@@ -124,3 +124,46 @@ def test_a_step_that_is_refused_can_be_made_again(sharded):
         assert [int(s["step"]) for s in opt.state_dict()["state"].values()] == [2, 3, 3]
     for a, b in zip(*runs):
         assert_bits_equal(a, b, "with and without refused steps")
+
+
+def _net(gen):
+    model = nn.Module()
+    model.inner = nn.Module()
+    for module, name, n in ((model.inner, "a", 300), (model.inner, "b", 77), (model, "c", 100), (model, "d", 513)):
+        module.register_parameter(name, nn.Parameter(torch.randn(n, device=DEV, generator=gen)))
+    return model
+
+
+@pytest.mark.parametrize("where", ["c", "inner.b"])
+@pytest.mark.parametrize("kind", ["gradient", "parameter"])
+@pytest.mark.parametrize("late", [False, True])
+def test_a_scale_inside_what_the_step_writes(where, kind, late):
+    """Sharded and plain parameters are all stepped with the value from before the step; with ``late``, one plain
+    parameter's count is behind, so that it is stepped by a launch of its own."""
+    from yafsdp_amd import MixedPrecisionPolicy, fully_shard
+    from yafsdp_amd.optim import FlatAdamW
+
+    runs = []
+    for apart in (True, False):
+        gen = torch.Generator(device=DEV).manual_seed(6)
+        model = _net(gen)
+        fully_shard(model.inner, mesh=(1, 0), mp_policy=MixedPrecisionPolicy(param_dtype=torch.bfloat16))
+        named = dict(model.named_parameters())
+        opt = FlatAdamW(named.values(), **HP)
+        for it in range(2):
+            for name, p in named.items():
+                fresh = torch.randn(loc(p).numel(), device=DEV, generator=gen)
+                if "inner" in name:
+                    p.grad = p._yafsdp_param().sharded_param_grad
+                    p.grad._local_tensor.copy_(fresh)
+                else:
+                    p.grad = None if late and it == 0 and name == "d" else fresh
+            p = named[where]
+            scale = loc(p.grad if kind == "gradient" else p)[5:6]
+            with torch.no_grad():
+                scale.fill_(0.375)
+            opt.step(grad_scale=scale.clone() if apart else scale, zero_grad=True)
+            assert all(p.grad is None or not loc(p.grad).any() for p in named.values())
+        runs.append([loc(p).clone() for p in named.values()])
+    for name, a, b in zip(named, *runs):
+        assert_bits_equal(a, b, f"{name}: scale apart and in the {kind} of {where}")

@@ -1,6 +1,6 @@
 """What the list passes and FlatAdamW promise around the arithmetic, as far as it can be checked without a GPU: which
 tensors they take for what, which memory a call may share, what a
-refused step leaves."""
+refused step leaves, where a gradient scale may lie."""
 
 import types
 import weakref
@@ -150,3 +150,55 @@ def test_a_refused_step_leaves_the_counts(monkeypatch):
     units = _plain_units(params, [torch.ones(4), None, torch.ones(4), torch.ones(4)], steps)
     opt._step_plain(units, HYPER, None, False)
     assert [u.steps[0] for u in units] == [4, 3, 1, 8]
+
+
+# ---- a gradient scale in memory that the step writes -------------------------------------------------------------
+def _shares(a, b):
+    lo, hi = a.data_ptr(), a.data_ptr() + 4 * a.numel()
+    return lo < b.data_ptr() + 4 * b.numel() and b.data_ptr() < hi
+
+
+def _stand_ins(monkeypatch, calls):
+    """The two native calls on CPU tensors with p -= scale * g as the step: the scale is read when a launch runs, and a
+    list is refused where what it writes shares memory."""
+
+    def one(p, g, m, v, out16=None, *, grad_scale, zero_grad, **kwargs):
+        p.sub_(grad_scale.clone() * g)
+        if zero_grad:
+            g.zero_()
+
+    def many(ps, gs, ms, vs, outs, resolve, *, grad_scale, zero_grad, **kwargs):
+        written = [*ps, *ms, *vs, *(gs if zero_grad else ())]
+        pairs = [(a, b) for i, a in enumerate(written) for b in written[:i]] + [(a, grad_scale) for a in written]
+        calls.append(not any(_shares(a, b) for a, b in pairs))
+        if calls[-1]:
+            for p, g, m, v in zip(ps, gs, ms, vs):
+                one(p, g, m, v, grad_scale=grad_scale, zero_grad=zero_grad)
+        return calls[-1]
+
+    monkeypatch.setattr(_native, "list_adamw", many)
+    monkeypatch.setattr(_native, "adamw_step", one)
+
+
+@pytest.mark.parametrize("where", ["gradient", "parameter", "elsewhere"])
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("steps", [[0, 0, 0], [1, 0, 0], [0, 1, 2]])
+@torch.no_grad()
+def test_a_scale_inside_what_the_step_writes(monkeypatch, where, shared, steps):
+    """Every parameter is stepped with the value from before the step."""
+    calls = []
+    _stand_ins(monkeypatch, calls)
+    base = torch.arange(12.0) + 1
+    params = [base[:4], base[4:8], base[6:10] if shared else base[8:]]
+    grads = [torch.full((4,), 0.5) for _ in params]
+    scale = {"gradient": grads[0][1:2], "parameter": params[0][2:3], "elsewhere": torch.tensor([0.5])}[where]
+    want, value = base.clone(), float(scale)
+    for p, g in zip(params, grads):
+        want[p.storage_offset():p.storage_offset() + 4] -= value * 0.5
+    opt = object.__new__(optim.FlatAdamW)
+    after = opt._step_plain(_plain_units(params, grads, steps), HYPER, scale, True)
+    assert torch.equal(base, want)
+    assert all(not g.any() for g in grads) and float(after) == value
+    assert (after is scale) == (where == "elsewhere")
+    if where == "elsewhere" and not shared:
+        assert calls == [True] * len(set(steps))

@@ -390,6 +390,16 @@ def list_adamw_step(
     )
 
 
+def _kept_apart(scalar: torch.Tensor, written: Iterable[torch.Tensor]) -> torch.Tensor:
+    """``scalar``, or a copy of it where it lies in one of the tensors that are about to be written."""
+    at = scalar.data_ptr()
+    for t in written:
+        lo = t.data_ptr()
+        if lo < at + scalar.element_size() and at < lo + t.numel() * t.element_size():
+            return scalar.clone()
+    return scalar
+
+
 class _Unit:
     """The parameters of one optimizer param group that live in one flat shard
     (an fsdp parameter group), or one plain tensor outside any group."""
@@ -501,7 +511,8 @@ class FlatAdamW(torch.optim.Optimizer):
         """One optimizer step.  ``grad_scale`` (one-element float32 device tensor,
         e.g. the coefficient from ``grad_clip_coef``) multiplies every gradient
         first, as a preceding ``grad.mul_`` would, without writing it back;
-        ``zero_grad=True`` zero-fills the gradients in the same pass."""
+        ``zero_grad=True`` zero-fills the gradients in the same pass.  A scale
+        that lies in memory the step writes counts with its value before it."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -517,12 +528,14 @@ class FlatAdamW(torch.optim.Optimizer):
                 if unit.group is None:
                     plain.append(unit)
                 else:
-                    self._step_unit(unit, hyper, grad_scale, zero_grad)
+                    grad_scale = self._step_unit(unit, hyper, grad_scale, zero_grad)
             if plain:
-                self._step_plain(plain, hyper, grad_scale, zero_grad)
+                grad_scale = self._step_plain(plain, hyper, grad_scale, zero_grad)
         return loss
 
-    def _step_plain(self, units: list[_Unit], hyper: dict[str, Any], grad_scale, zero_grad: bool) -> None:
+    # Either kind returns the gradient scale for what is stepped after it: a copy from the first launch on that writes
+    # the memory it lies in.
+    def _step_plain(self, units: list[_Unit], hyper: dict[str, Any], grad_scale, zero_grad: bool) -> torch.Tensor | None:
         """Parameters outside any group: one list pass per GPU and step count."""
         live = [(unit, unit.params[0], unit.params[0].grad) for unit in units if unit.params[0].grad is not None]
         for _, _, grad in live:
@@ -534,9 +547,15 @@ class FlatAdamW(torch.optim.Optimizer):
         for (_, step), run in runs.items():
             lists = ([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
                      [u.exp_avg_sq for u, _, _ in run])
+            how = dict(hyper, step=step, zero_grad=zero_grad, bump_versions=False, allow_overlap=True)
+            taken = _native.list_adamw(*lists, None, _resolve, grad_scale=grad_scale, **how)
+            if not taken and grad_scale is not None:
+                apart = _kept_apart(grad_scale, (t for k, ts in enumerate(lists) if k != 1 or zero_grad for t in ts))
+                if apart is not grad_scale:
+                    grad_scale = apart
+                    taken = _native.list_adamw(*lists, None, _resolve, grad_scale=grad_scale, **how)
             # a count advances once its launch has been accepted: what a refused call leaves can be stepped again
-            if _native.list_adamw(*lists, None, _resolve, step=step, grad_scale=grad_scale, zero_grad=zero_grad,
-                                  bump_versions=False, allow_overlap=True, **hyper):
+            if taken:
                 for unit, _, _ in run:
                     unit.steps[0] = step
                 continue
@@ -545,21 +564,22 @@ class FlatAdamW(torch.optim.Optimizer):
                 _native.adamw_step(p.view(-1), grad.view(-1), unit.exp_avg, unit.exp_avg_sq, None, step=step,
                                    grad_scale=grad_scale, zero_grad=zero_grad, **hyper)
                 unit.steps[0] = step
+        return grad_scale
 
-    def _step_unit(self, unit: _Unit, hyper: dict[str, Any], grad_scale, zero_grad: bool) -> None:
+    def _step_unit(self, unit: _Unit, hyper: dict[str, Any], grad_scale, zero_grad: bool) -> torch.Tensor | None:
         group = unit.group
         key = unit.key
         shard = group._padded_sharded_param_data[key]
         grad_shard = group._padded_sharded_param_grad[key]
         if grad_shard is None:
-            return
+            return grad_scale
         class_params = group._all_gather_dtype_to_fsdp_params[key]
         # launches: maximal runs of fragments that have a gradient and share a step count
         ranges = _grad_ranges(group, unit.indices, key)
         whole = ranges == [(0, shard.numel())]
         with_grad = [k for k, p in enumerate(unit.params) if p.grad is not None]
         if not with_grad:
-            return
+            return grad_scale
         steps = {k: unit.steps[k] + 1 for k in with_grad}
         uniform = len(set(steps.values())) == 1
         # the fused copy-in needs the whole shard rewritten in this pass; otherwise the
@@ -582,6 +602,8 @@ class FlatAdamW(torch.optim.Optimizer):
                         runs.append((lo, hi, steps[k]))
         if zero_grad:
             group._grad_sumsq_token.pop(key, None)  # the gradients are rewritten
+        if grad_scale is not None:
+            grad_scale = _kept_apart(grad_scale, (shard, unit.exp_avg, unit.exp_avg_sq, *((grad_shard,) if zero_grad else ())))
         for lo, hi, step in runs:
             _native.adamw_step(
                 shard[lo:hi], grad_shard[lo:hi], unit.exp_avg[lo:hi], unit.exp_avg_sq[lo:hi],
@@ -596,6 +618,7 @@ class FlatAdamW(torch.optim.Optimizer):
                 fsdp_param.set_all_gather_input()
             group._all_gather_input_set_dtypes.add(None)
             group._copy_in_shard_version = shard._version
+        return grad_scale
 
     # --------------------------------------------------------------- state dicts --
     def state_dict(self) -> dict[str, Any]:
