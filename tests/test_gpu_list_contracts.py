@@ -167,3 +167,28 @@ def test_a_scale_inside_what_the_step_writes(where, kind, late):
         runs.append([loc(p).clone() for p in named.values()])
     for name, a, b in zip(named, *runs):
         assert_bits_equal(a, b, f"{name}: scale apart and in the {kind} of {where}")
+
+
+@pytest.mark.parametrize("make", [
+    lambda: PairTensor(*(torch.full((1,), 0.5, device=DEV) for _ in range(2))),
+    lambda: torch._efficientzerotensor(1, device=DEV),
+    lambda: torch.full((1,), 0.5j, device=DEV, dtype=torch.complex64).conj().imag,
+])
+def test_a_scale_without_a_value_in_memory_is_refused(make):
+    """A wrapper and a zero without storage (address 0, "no scale" to the library); a lazily negated view (the other sign
+    in memory)."""
+    from yafsdp_amd import _native
+    from yafsdp_amd.optim import FlatAdamW, list_adamw_step, list_scale_grads_
+
+    p, g, m, v = (torch.ones(10, device=DEV) for _ in range(4))
+    param = nn.Parameter(p)
+    param.grad = g
+    opt = FlatAdamW([param], **HP)
+    for call in (lambda c: list_adamw_step([p], [g], [m], [v], step=1, grad_scale=c), lambda c: opt.step(grad_scale=c),
+                 lambda c: list_scale_grads_([g], c), lambda c: _native.flat_scale(g, c),
+                 lambda c: _native.adamw_step(p, g, m, v, None, lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8,
+                                              weight_decay=0.0, step=1, grad_scale=c)):
+        with pytest.raises(TypeError, match="must hold its value in memory"):
+            call(make())
+    for t in (p, g, m, v):
+        assert_bits_equal(t, torch.ones(10), "a refused call writes nothing")

@@ -202,3 +202,13 @@ def test_a_scale_inside_what_the_step_writes(monkeypatch, where, shared, steps):
     assert (after is scale) == (where == "elsewhere")
     if where == "elsewhere" and not shared:
         assert calls == [True] * len(set(steps))
+
+
+def test_a_scale_without_memory_of_its_own_is_refused():
+    """Its address is 0, which the library takes for "no scale"."""
+    scale = PairTensor(torch.full((1,), 0.5), torch.full((1,), 0.5), "cuda")
+    four = [[torch.zeros(2)] for _ in range(4)]
+    with pytest.raises(TypeError, match="grad_scale must hold its value"):
+        optim.list_adamw_step(*four, step=1, grad_scale=scale)
+    with pytest.raises(TypeError, match="coef must hold its value"):
+        optim.list_scale_grads_(four[0], scale)

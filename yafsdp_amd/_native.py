@@ -237,6 +237,18 @@ def _flat_arg(t: torch.Tensor, what: str) -> torch.Tensor:
     return t
 
 
+def _scalar_arg(t: torch.Tensor, what: str, whose: str, device: "torch.device | None" = None) -> int:
+    """Address of a factor that a kernel reads: a tensor without memory of its own has none (NULL means "no factor" to
+    some entry points), and that of a lazily negated view holds the other sign."""
+    _flat_arg(t, what)
+    if t.dtype != torch.float32 or t.numel() != 1 or (device is not None and t.device != device):
+        raise TypeError(f"{what} must be a one-element float32 tensor on the {whose} device")
+    address = t.data_ptr()
+    if not address or t.is_neg():
+        raise TypeError(f"{what} must hold its value in memory of its own, got a {type(t).__name__} that does not")
+    return address
+
+
 _raw_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _NO_SWITCH = contextlib.nullcontext()
 
@@ -872,11 +884,10 @@ def clip_coef(sumsq: torch.Tensor, max_norm: float, norm_and_coef: torch.Tensor)
 
 def flat_scale(buf: torch.Tensor, coef: torch.Tensor) -> None:
     """``buf.mul_(coef)`` with a one-element float32 device tensor; a coefficient of exactly 1 costs no traffic."""
-    _flat_arg(buf, "buf"), _flat_arg(coef, "coef")
-    if coef.dtype != torch.float32 or coef.numel() != 1 or coef.device != buf.device:
-        raise TypeError("coef must be a one-element float32 tensor on the buffer's device")
+    _flat_arg(buf, "buf")
+    coef_ptr = _scalar_arg(coef, "coef", "buffer's", buf.device)
     with _on(buf.device):
-        _check(lib.yafsdp_flat_scale(buf.data_ptr(), _dt(buf), buf.numel(), coef.data_ptr(), _stream(buf)), "yafsdp_flat_scale")
+        _check(lib.yafsdp_flat_scale(buf.data_ptr(), _dt(buf), buf.numel(), coef_ptr, _stream(buf)), "yafsdp_flat_scale")
 
 
 def adamw_step(
@@ -910,12 +921,7 @@ def adamw_step(
         if out16.dtype not in (torch.bfloat16, torch.float16) or out16.numel() != n or out16.device != param.device:
             raise TypeError("out16 must be a bfloat16 / float16 tensor of the shard's size on its device")
         out_ptr, out_dt = out16.data_ptr(), _dt(out16)
-    gs_ptr = None
-    if grad_scale is not None:
-        _flat_arg(grad_scale, "grad_scale")
-        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != param.device:
-            raise TypeError("grad_scale must be a one-element float32 tensor on the shard's device")
-        gs_ptr = grad_scale.data_ptr()
+    gs_ptr = None if grad_scale is None else _scalar_arg(grad_scale, "grad_scale", "shard's", param.device)
     flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
     with _on(param.device):
         _check(
@@ -1081,14 +1087,14 @@ def list_clip(tensors, norm_type, max_norm: float, what: str = "tensors", resolv
 
 def list_scale(tensors, coef: torch.Tensor, what: str = "tensors", resolve=None) -> None:
     """``t.mul_(coef)`` for every tensor of a list (see ``TensorList``), ``coef`` a one-element float32 device tensor."""
-    _flat_arg(coef, "coef")
+    coef_ptr = _scalar_arg(coef, "coef", "list's")
     lst = TensorList(tensors, what, resolve)
-    if coef.dtype != torch.float32 or coef.numel() != 1 or coef.device != lst.device:
+    if coef.device != lst.device:
         raise TypeError("coef must be a one-element float32 tensor on the list's device")
     workspace, nbytes = _list_workspace(lst)
     with _on(lst.device):
         _check(
-            lib.yafsdp_list_scale(lst.entries, lst.count, coef.data_ptr(), workspace.data_ptr(), nbytes,
+            lib.yafsdp_list_scale(lst.entries, lst.count, coef_ptr, workspace.data_ptr(), nbytes,
                                   _device_stream(lst.device)),
             "yafsdp_list_scale",
         )
@@ -1160,12 +1166,7 @@ def list_adamw(
     """One Adam(W) step on every position of the lists (see ``AdamwList``), with the bits of ``adamw_step``.  Tensors that
     the step writes must not share memory: refused, or with ``allow_overlap`` reported by returning False with nothing
     launched."""
-    gs_ptr = 0
-    if grad_scale is not None:
-        _flat_arg(grad_scale, "grad_scale")
-        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
-            raise TypeError("grad_scale must be a one-element float32 tensor on the parameters' device")
-        gs_ptr = grad_scale.data_ptr()
+    gs_ptr = 0 if grad_scale is None else _scalar_arg(grad_scale, "grad_scale", "parameters'")
     flags = (ADAM_DECOUPLED_DECAY if decoupled else 0) | (ADAM_ZERO_GRAD if zero_grad else 0)
     lists = [_as_list(ts, name) for ts, name in zip((params, grads, exp_avgs, exp_avg_sqs), AdamwList._NAMES)]
     lists.append(None if outs16 is None else _as_list(outs16, "outs16"))
