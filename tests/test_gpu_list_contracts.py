@@ -192,3 +192,31 @@ def test_a_scale_without_a_value_in_memory_is_refused(make):
             call(make())
     for t in (p, g, m, v):
         assert_bits_equal(t, torch.ones(10), "a refused call writes nothing")
+
+
+# ---- an older error of the thread --------------------------------------------------------------------------------
+@pytest.mark.parametrize("count", [3, 400])  # in the kernel arguments, through a staging slot
+def test_an_error_of_an_earlier_call_is_not_the_launches(count):
+    """A HIP error that another call of the thread left behind: the list calls report their own launches' status, run to
+    their end and leave it for whoever asks.  More calls than staging slots, none of which may be given up early."""
+    from yafsdp_amd import _native
+    from yafsdp_amd.optim import list_clip_coef
+
+    lib = _native.lib
+    lists = [[torch.full((5 + k,), float(k + 1), device=DEV) for _ in range(count)] for k in range(40)]
+    want = [torch.stack(list_clip_coef(ts, 1.0)) for ts in lists]
+    entries = [_native.TensorList(ts) for ts in lists]
+    nbytes = lib.yafsdp_list_workspace_bytes(count)
+    workspaces = [torch.empty(nbytes, dtype=torch.uint8, device=DEV) for _ in lists]
+    got = torch.zeros(len(lists), 2, device=DEV)
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.hipPeekAtLastError() == 0
+    older = lib.hipSetDevice(1 << 20)
+    assert older != 0 and lib.hipPeekAtLastError() == older
+    codes = [lib.yafsdp_list_norm(e.entries, e.count, 2, 1.0, w.data_ptr(), nbytes, got[k].data_ptr(), stream)
+             for k, (e, w) in enumerate(zip(entries, workspaces))]
+    left = lib.hipGetLastError()
+    torch.cuda.synchronize()
+    assert codes == [0] * len(lists) and left == older
+    assert_bits_equal(got, torch.stack(want), "norms and coefficients")

@@ -24,17 +24,22 @@ struct TimedLaunch {
 };
 extern thread_local TimedLaunch tl_timed_launch;
 
+// The status is the launch's own: the thread's last error may be that of an older call, with the kernel queued all the same.
+// It is left as it was, except that a failed launch's is taken back (the caller gets it).
 template <class... Params, class... Args>
 inline hipError_t launch_kernel(void (*kernel)(Params...), int grid, int block, hipStream_t stream, Args... args) {
-  TimedLaunch& t = tl_timed_launch;
-  if (t.start != nullptr || t.stop != nullptr) {
-    const hipEvent_t a = t.start, b = t.stop;
+  const auto go = [&](Params... p) {
+    void* a[] = {const_cast<void*>(static_cast<const void*>(&p))...};
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    TimedLaunch& t = tl_timed_launch;
+    if (t.start == nullptr && t.stop == nullptr) return hipLaunchKernel(fn, dim3(grid), dim3(block), a, 0, stream);
+    const hipEvent_t start = t.start, stop = t.stop;
     t.start = t.stop = nullptr;
-    hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(block), 0, stream, a, b, 0, static_cast<Params>(args)...);
-  } else {
-    kernel<<<dim3(grid), dim3(block), 0, stream>>>(static_cast<Params>(args)...);
-  }
-  return hipGetLastError();
+    return hipExtLaunchKernel(fn, dim3(grid), dim3(block), a, 0, stream, start, stop, 0);
+  };
+  const hipError_t e = go(static_cast<Params>(args)...);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
 }
 
 // dst[i] = post_elem(src[i], dst[i]); scale is SCALE_NONE / SCALE_MUL / SCALE_DIV

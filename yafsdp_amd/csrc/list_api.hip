@@ -159,8 +159,9 @@ bool have_slots(StageSlots& s) {
     if (hipHostMalloc(&block, StageSlots::kBlockBytes, hipHostMallocPortable | hipHostMallocMapped | hipHostMallocCoherent) ==
         hipSuccess)
       s.attach(block);
+    else
+      (void)hipGetLastError();  // without pinned memory the other route serves
     if (exchanged) (void)hipThreadExchangeStreamCaptureMode(&mode);
-    (void)hipGetLastError();  // without pinned memory the other route serves
   }
   return s.attached();
 }
