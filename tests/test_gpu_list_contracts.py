@@ -220,3 +220,31 @@ def test_an_error_of_an_earlier_call_is_not_the_launches(count):
     torch.cuda.synchronize()
     assert codes == [0] * len(lists) and left == older
     assert_bits_equal(got, torch.stack(want), "norms and coefficients")
+
+
+# ---- order -----------------------------------------------------------------------------------------------------
+def test_shared_memory_across_step_counts():
+    """Three parameters on one storage, the middle one a step behind: stepped in the list's order, as one launch per
+    parameter steps them."""
+    from oracle import cref
+    from yafsdp_amd.optim import FlatAdamW
+
+    chp = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1)
+    gen = torch.Generator().manual_seed(8)
+    want = torch.randn(100, generator=gen)
+    base = want.to(DEV)
+    cuts = [slice(0, 60), slice(40, 90), slice(72, 100)]
+    params = [nn.Parameter(base[c]) for c in cuts]
+    state = [[torch.zeros(c.stop - c.start) for c in cuts] for _ in range(2)]
+    opt, counts = FlatAdamW(params, **HP), [0, 0, 0]
+    for it in range(3):
+        for k, (p, c) in enumerate(zip(params, cuts)):
+            g = torch.randn(c.stop - c.start, generator=gen)
+            p.grad = None if (it, k) == (0, 1) else g.to(DEV)
+            if p.grad is not None:
+                counts[k] += 1
+                part = want[c].clone()
+                cref.adamw_step(part, g, state[0][k], state[1][k], None, step=counts[k], **chp)
+                want[c] = part
+        opt.step()
+        assert_bits_equal(base, want, f"after step {it}")

@@ -1,6 +1,6 @@
 """What the list passes and FlatAdamW promise around the arithmetic, as far as it can be checked without a GPU: which
 tensors they take for what, which memory a call may share, what a
-refused step leaves, where a gradient scale may lie."""
+refused step leaves, where a gradient scale may lie, in which order parameters are stepped."""
 
 import types
 import weakref
@@ -212,3 +212,37 @@ def test_a_scale_without_memory_of_its_own_is_refused():
         optim.list_adamw_step(*four, step=1, grad_scale=scale)
     with pytest.raises(TypeError, match="coef must hold its value"):
         optim.list_scale_grads_(four[0], scale)
+
+
+# ---- order -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("steps", [[0, 0, 0, 0], [1, 0, 1, 0], [2, 1, 0, 3]])
+@pytest.mark.parametrize("what", ["nothing", "parameters", "gradients", "gradients that are read"])
+@torch.no_grad()
+def test_memory_shared_across_step_counts_keeps_the_lists_order(monkeypatch, steps, what):
+    """Parameters (or zero-filled gradients) that share memory are stepped in the list's order whatever their counts;
+    others go in one pass per count."""
+    _stand_ins(monkeypatch, [])
+    order, many = [], _native.list_adamw
+    base = torch.arange(16.0)
+    params = [base[k:k + 5] if what == "parameters" else base[4 * k:4 * k + 4] for k in range(4)]
+    shared = torch.ones(4)
+    grads = [shared if what.startswith("gradients") else torch.ones(p.numel()) for p in params]
+    at = [p.data_ptr() for p in params]
+
+    def watch(ps, *args, **kwargs):
+        taken = many(ps, *args, **kwargs)
+        order.extend([at.index(p.data_ptr()) for p in ps] if taken else ())
+        return taken
+
+    def watch_one(p, *args, **kwargs):
+        order.append(at.index(p.data_ptr()))
+
+    monkeypatch.setattr(_native, "list_adamw", watch)
+    monkeypatch.setattr(_native, "adamw_step", watch_one)
+    units = _plain_units(params, grads, steps)
+    object.__new__(optim.FlatAdamW)._step_plain(units, HYPER, torch.tensor([0.5]), what != "gradients that are read")
+    if what in ("parameters", "gradients"):
+        assert order == [0, 1, 2, 3]
+    else:
+        assert order == sorted(range(4), key=lambda k: (steps.index(steps[k]), k))
+    assert [u.steps[0] for u in units] == [s + 1 for s in steps]

@@ -400,6 +400,12 @@ def _kept_apart(scalar: torch.Tensor, written: Iterable[torch.Tensor]) -> torch.
     return scalar
 
 
+def _any_shared(tensors: Iterable[torch.Tensor]) -> bool:
+    """Whether two of these dense tensors share a byte."""
+    spans = sorted((lo := t.data_ptr(), lo + t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 class _Unit:
     """The parameters of one optimizer param group that live in one flat shard
     (an fsdp parameter group), or one plain tensor outside any group."""
@@ -523,20 +529,19 @@ class FlatAdamW(torch.optim.Optimizer):
             beta1, beta2 = pg["betas"]
             hyper = dict(lr=float(pg["lr"]), beta1=beta1, beta2=beta2, eps=pg["eps"],
                          weight_decay=pg["weight_decay"], decoupled=pg["decoupled_weight_decay"])
-            plain: list[_Unit] = []
-            for unit in self._units_of(pg_index, pg):
-                if unit.group is None:
-                    plain.append(unit)
-                else:
-                    grad_scale = self._step_unit(unit, hyper, grad_scale, zero_grad)
+            units = self._units_of(pg_index, pg)  # those outside any group first
+            plain = [unit for unit in units if unit.group is None]
             if plain:
                 grad_scale = self._step_plain(plain, hyper, grad_scale, zero_grad)
+            for unit in units[len(plain):]:
+                grad_scale = self._step_unit(unit, hyper, grad_scale, zero_grad)
         return loss
 
     # Either kind returns the gradient scale for what is stepped after it: a copy from the first launch on that writes
     # the memory it lies in.
     def _step_plain(self, units: list[_Unit], hyper: dict[str, Any], grad_scale, zero_grad: bool) -> torch.Tensor | None:
-        """Parameters outside any group: one list pass per GPU and step count."""
+        """Parameters outside any group: one list pass per GPU and step count (parameters that share memory across step
+        counts: one each, in the list's order)."""
         live = [(unit, unit.params[0], unit.params[0].grad) for unit in units if unit.params[0].grad is not None]
         for _, _, grad in live:
             if grad.dtype != torch.float32 or not grad.is_contiguous():
@@ -544,7 +549,10 @@ class FlatAdamW(torch.optim.Optimizer):
         runs: dict[tuple[torch.device, int], list[tuple[_Unit, torch.Tensor, torch.Tensor]]] = {}
         for unit, p, grad in live:
             runs.setdefault((unit.device, unit.steps[0] + 1), []).append((unit, p, grad))
-        for (_, step), run in runs.items():
+        passes = [(step, run) for (_, step), run in runs.items()]
+        if len(passes) > 1 and _any_shared(t for _, p, g in live for t in ((p, g) if zero_grad else (p,))):
+            passes = [(entry[0].steps[0] + 1, [entry]) for entry in live]
+        for step, run in passes:
             lists = ([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
                      [u.exp_avg_sq for u, _, _ in run])
             how = dict(hyper, step=step, zero_grad=zero_grad, bump_versions=False, allow_overlap=True)
