@@ -248,3 +248,45 @@ def test_shared_memory_across_step_counts():
                 want[c] = part
         opt.step()
         assert_bits_equal(base, want, f"after step {it}")
+
+
+# ---- one norm over the ranks -------------------------------------------------------------------------------------
+def test_norm_of_fragments_and_replicated_gradients_joined_over_ranks():
+    """Two logical ranks of a model with sharded and replicated parameters: the squares of the fragments' norms are summed
+    over the ranks, those of the replicated gradients counted once; every rank clips by the coefficient of the whole
+    gradient.  Each of the six roundings to binary32 on the way is off by at most 2^-24 of the norm."""
+    from yafsdp_amd import MixedPrecisionPolicy, fully_shard
+    from yafsdp_amd._tensor import RaggedShardDTensor
+    from yafsdp_amd.optim import list_grad_norm, list_scale_grads_
+
+    max_norm, squares, ranks, whole = 0.5, [], [], None
+    for rank in range(2):
+        gen = torch.Generator(device=DEV).manual_seed(9)
+        model = _net(gen)
+        full = {k: torch.randn(p.shape, device=DEV, generator=gen) for k, p in model.named_parameters()}
+        whole = torch.cat([g.view(-1) for g in full.values()]).double()
+        fully_shard(model.inner, mesh=(2, rank), mp_policy=MixedPrecisionPolicy(param_dtype=torch.bfloat16))
+        for name, p in model.named_parameters():
+            if isinstance(p, RaggedShardDTensor):
+                p.grad = p._yafsdp_param().sharded_param_grad
+                at = p.placements[0]
+                p.grad._local_tensor.copy_(full[name][at.global_offset:at.global_offset + at.local_numel])
+            else:
+                p.grad = full[name]
+        grads = [p.grad for p in model.parameters()]
+        sharded = [g for g in grads if isinstance(g, RaggedShardDTensor)]
+        plain = [g for g in grads if not isinstance(g, RaggedShardDTensor)]
+        squares.append(list_grad_norm(sharded).double().square())
+        ranks.append((grads, list_grad_norm(plain).double().square()))
+    before = [[loc(g).clone() for g in grads] for grads, _ in ranks]
+    coefs = []
+    for grads, replicated in ranks:
+        total_norm = (sum(squares) + replicated).sqrt().float()
+        coefs.append((max_norm / (total_norm + 1e-6)).clamp(max=1.0))
+        assert abs(total_norm.item() - whole.norm().item()) <= 6 * 2.0 ** -24 * whole.norm().item()
+        list_scale_grads_(grads, coefs[-1])
+    assert_bits_equal(coefs[0], coefs[1], "one coefficient on all ranks")
+    assert coefs[0].item() < 1.0
+    for (grads, _), olds in zip(ranks, before):
+        for g, old in zip(grads, olds):
+            assert_bits_equal(loc(g), old * coefs[0], "clipped fragment")

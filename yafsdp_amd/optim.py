@@ -325,11 +325,13 @@ def list_clip_coef(
     ``FlatAdamW.step`` to fuse the scaling into the optimizer pass.
 
     ``grads`` may mix float32, bfloat16 and float16; ``None`` entries (parameters without a gradient) are left out, and
-    a sharded gradient counts with this rank's fragment.  Each is dense in memory, all live on one GPU; any other tensor
-    subclass that keeps its values in inner tensors is refused.  ``norm_type``
-    is 1, 2 or infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64
-    and are reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls;
-    the call can be captured into a HIP graph, which then reads the same addresses at every replay."""
+    a sharded gradient counts with this rank's fragment alone: the norm and coefficient of a list that holds one are this
+    rank's, to be joined with the other ranks' before anything is scaled.  A list without a tensor raises ValueError
+    (torch's functions return 0): nothing says where the result should live.  Each tensor is dense in memory, all live on
+    one GPU; any other tensor subclass that keeps its values in inner tensors is refused.  ``norm_type`` is 1, 2 or
+    infinity over all elements of all tensors; a NaN makes both results NaN.  The sums are held in binary64 and are
+    reproducible for the same tensors at the same addresses.  No host synchronisation, no state between calls; the call
+    can be captured into a HIP graph, which then reads the same addresses at every replay."""
     return _native.list_norm(grads, norm_type, max_norm, "grads", _resolve).unbind()
 
 
@@ -343,7 +345,8 @@ def list_clip_grad_norm_(
 ) -> torch.Tensor:
     """``torch.nn.utils.clip_grad_norm_`` over a list of gradients (see ``list_clip_coef``): every element is multiplied
     by the clip coefficient in binary32 and rounded to its tensor's dtype, in place; returns the total norm.  Nothing is
-    written when nothing is clipped.  The tensors must not share memory."""
+    written when nothing is clipped.  The tensors must not share memory.  For gradients that all live on this rank: with
+    fragments of several ranks in play, join the norms and use ``list_scale_grads_``."""
     return _native.list_clip(grads, norm_type, max_norm, "grads", _resolve)[0]
 
 
