@@ -246,3 +246,22 @@ def test_memory_shared_across_step_counts_keeps_the_lists_order(monkeypatch, ste
     else:
         assert order == sorted(range(4), key=lambda k: (steps.index(steps[k]), k))
     assert [u.steps[0] for u in units] == [s + 1 for s in steps]
+
+
+@pytest.mark.parametrize("helper", [True, False])
+def test_any_shared(helper, monkeypatch):
+    if helper:
+        tl = pytest.importorskip("yafsdp_amd._tensorlist")
+        assert tl.any_shared([torch.zeros(2), torch.zeros(8)[::2]]) is None  # handed back: not dense, not plain
+        assert tl.any_shared([Int8Master(torch.zeros(2))]) is None and tl.any_shared(iter([])) is None
+    else:
+        monkeypatch.setattr(_native, "_tensorlist", None)
+    base = torch.zeros(100)
+    far, half = torch.zeros(5), torch.zeros(6, dtype=torch.bfloat16)
+    cut = lambda *spans: [base[a:b] for a, b in spans]
+    for tensors, shared in ((cut((50, 60), (0, 10), (10, 50)), False), (cut((50, 60), (0, 10), (9, 50)), True),
+                            (cut((0, 100), (30, 40)), True), ([base, base], True), ([], False), ([far, half, base], False),
+                            ([half, half[5:]], True), ([half[:5], half[5:]], False), (cut((3, 3), (0, 10), (3, 3)), False),
+                            ([base.view(10, 10).t(), torch.nn.Parameter(base[99:])], True)):
+        assert _native.any_shared(tensors) is shared
+    assert not _native.any_shared([PairTensor(far, far, "cuda"), Int8Master(far)])  # no memory of their own

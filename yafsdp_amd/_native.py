@@ -1027,6 +1027,15 @@ def _bump_versions(tensors, where=None) -> None:
     torch.autograd.graph.increment_version([t for t in live if not t.is_inference()])
 
 
+def any_shared(tensors: "list[torch.Tensor]") -> bool:
+    """Whether two of these tensors share a byte of the memory from their first element on."""
+    got = _tensorlist.any_shared(tensors) if _tensorlist is not None else None
+    if got is not None:
+        return got
+    spans = sorted((at := t.data_ptr(), at + t.numel() * t.element_size()) for t in tensors if t.numel() and t.data_ptr())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 def norm_code(norm_type) -> int:
     try:
         return NORM_CODE[float(norm_type)]

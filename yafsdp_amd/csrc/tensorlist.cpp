@@ -13,7 +13,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <utility>
 #include <vector>
 
 #include "../../include/yafsdp_hip.h"
@@ -218,6 +220,29 @@ void bump_versions(py::handle tensors, py::handle where) {
   }
 }
 
+// Whether two tensors of the list share a byte (0.3 us per tensor in Python); None if the list holds anything but plain
+// dense tensors.
+py::object any_shared(py::handle tensors) {
+  PyObject* seq = tensors.ptr();
+  if (!PyList_Check(seq) && !PyTuple_Check(seq)) return py::none();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  PyObject** items = PySequence_Fast_ITEMS(seq);
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  spans.reserve(size_t(n));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!THPVariable_CheckExact(items[i])) return py::none();
+    const at::Tensor& t = THPVariable_Unpack(items[i]);
+    if (t.layout() != at::kStrided || !t.is_non_overlapping_and_dense()) return py::none();
+    if (t.numel() == 0) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    spans.emplace_back(at, at + t.nbytes());
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i - 1].second > spans[i].first) return py::bool_(true);
+  return py::bool_(false);
+}
+
 // ---- whole calls, for lists on the current device ---------------------------------------------------------------
 // What the Python binding does through ctypes in 5-6 us (entries as bytes, two torch.empty, argument conversion) takes
 // about 2 us here.  `fn` / `ws_fn`: addresses of the ABI's entry point and of its workspace size.
@@ -275,5 +300,6 @@ PYBIND11_MODULE(_tensorlist, m) {
   m.def("adamw_entries", &adamw_entries, "yafsdp_adamw_entry array of parallel lists of tensors");
   m.def("list_norm", &list_norm);
   m.def("list_adamw", &list_adamw);
+  m.def("any_shared", &any_shared);
   m.def("bump_versions", &bump_versions, py::arg("tensors"), py::arg("where") = py::none());
 }

@@ -403,12 +403,6 @@ def _kept_apart(scalar: torch.Tensor, written: Iterable[torch.Tensor]) -> torch.
     return scalar
 
 
-def _any_shared(tensors: Iterable[torch.Tensor]) -> bool:
-    """Whether two of these dense tensors share a byte."""
-    spans = sorted((lo := t.data_ptr(), lo + t.numel() * t.element_size()) for t in tensors if t.numel())
-    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
-
-
 class _Unit:
     """The parameters of one optimizer param group that live in one flat shard
     (an fsdp parameter group), or one plain tensor outside any group."""
@@ -553,7 +547,7 @@ class FlatAdamW(torch.optim.Optimizer):
         for unit, p, grad in live:
             runs.setdefault((unit.device, unit.steps[0] + 1), []).append((unit, p, grad))
         passes = [(step, run) for (_, step), run in runs.items()]
-        if len(passes) > 1 and _any_shared(t for _, p, g in live for t in ((p, g) if zero_grad else (p,))):
+        if len(passes) > 1 and _native.any_shared([p for _, p, _ in live] + [g for _, _, g in live if zero_grad]):
             passes = [(entry[0].steps[0] + 1, [entry]) for entry in live]
         for step, run in passes:
             lists = ([p for _, p, _ in run], [g for _, _, g in run], [u.exp_avg for u, _, _ in run],
@@ -614,7 +608,8 @@ class FlatAdamW(torch.optim.Optimizer):
         if zero_grad:
             group._grad_sumsq_token.pop(key, None)  # the gradients are rewritten
         if grad_scale is not None:
-            grad_scale = _kept_apart(grad_scale, (shard, unit.exp_avg, unit.exp_avg_sq, *((grad_shard,) if zero_grad else ())))
+            written = (shard, unit.exp_avg, unit.exp_avg_sq, grad_shard)
+            grad_scale = _kept_apart(grad_scale, written if zero_grad else written[:3])
         for lo, hi, step in runs:
             _native.adamw_step(
                 shard[lo:hi], grad_shard[lo:hi], unit.exp_avg[lo:hi], unit.exp_avg_sq[lo:hi],
