@@ -25,7 +25,7 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 HP = dict(lr=1e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
 CHP = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1)
 
-# around a 16-byte vector, a 128-byte line, a 4-KiB tile (1024 / 2048 elements) and AdamW's 512-element tile
+# around a 16-byte vector, a 128-byte line, a 4-KiB tile (1024 / 2048 elements) and two of AdamW's 256-element tiles
 EDGES = [1, 0, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 511, 512, 513, 1023, 1024, 1025, 2047, 2048,
          2049, 4095, 4097, 6001]
 

@@ -98,8 +98,9 @@ constexpr int kListClipTiles = 32768;
 // AdamW: one tile of 256 elements per wave, one wave per workgroup (a layer of 218 M elements, 6.1 GB: 1011 us; tiles
 // of 512 and 1024 elements 1038 and 1050; two and four waves per workgroup with tiles of 512 1051 and 1075).
 constexpr int kListAdamBlock = 64;
-// A grid has fewer than 2^32 lanes: a wave per tile takes several launches beyond this many (17 GB; 1.07 G elements of
-// AdamW).  (Waves that loop instead cost 0.4-1.5 % at every size.)
+// A wave per tile takes several launches beyond this many workgroups (17 GB of scaling; 1.07 G elements of AdamW): 2^28
+// lanes, a sixteenth of the 2^32 that a grid stays below.  Each is 5 ms of work, so the 5 us of one launch more are
+// 0.1 %, and lists that need several still fit a card.  (Waves that loop instead cost 0.4-1.5 % at every size.)
 constexpr uint32_t kListMaxGrid = 1u << 22;
 
 }  // namespace yafsdp

@@ -6,7 +6,7 @@
 // ranges measured slower: from the kernel arguments 97 us against 87 on 1427 tensors, because those are far away, and
 // from the workspace 74 against 69, because a vector load queues behind the data's.)
 //
-// Reached on MI355X (kernel alone): norm of 436 MB of bf16 6.7 TB/s and of 1.74 GB 6.9 TB/s (a read-only pass 7.2);
+// Reached on MI355X (kernel alone, traced): norm of 436 MB of bf16 6.5-6.7 TB/s and of 1.74 GB 7.0 TB/s (a read-only pass 7.2);
 // scaling 1.74 GB 6.3 TB/s (a copy 6.36); AdamW of 218 M elements 6.05 TB/s, with 573 ragged tensors 6.1 (a mover of its
 // streams without arithmetic 6.1-6.2).  What is left is the 4-5 us per launch that run below full rate.
 #pragma once
